@@ -19,7 +19,8 @@
  * legacy default stream, as in the reference; nothing throws; one thread per process.
  * Sticky error codes read by sl_check: 1..11 as in core/cuda/kernels.cu:21-34,101-108 (2 launch, 3 sync);
  * 12 bad argument, 13 compute on cpu, 14 device not initialised through sl_init_device,
- * 21/22/23 a bounded device-side wait on a peer rank ran out (start / reduced / done barrier).
+ * 21/22/23 a bounded device-side wait on a peer rank ran out (start / reduced / done barrier), 24 one inside a matrix
+ * product.
  */
 #ifndef SOLITON_B200_H
 #define SOLITON_B200_H
@@ -231,6 +232,66 @@ void slb_run_range(int64_t tiles, int world, int chunk, int blocks, int block, i
  * tensors, -3 a CUDA call failed. */
 int slb_adamw_step_static(int nseg, float* const* p, const float* const* g, float* const* m, float* const* v,
                           const int64_t* n, const float* wd, float lr, float b1, float b2, float eps, int step);
+/* ---- Feed-forward operators and 8-bit activation checkpoints. No counterpart in the reference.
+ *
+ * Tensors are dense row-major fp32 at any 4-byte alignment; weights are (features out, features in), a bias holds one
+ * value per feature out. Activations: 0 none, 1 GELU (exact, through erf), 2 SiLU. Work goes to the legacy default
+ * stream (so a call cannot be captured into a graph); nothing is kept from one call for the next; the same inputs give
+ * the same bits. Results 0, -1 (sticky error set: 12 bad argument, 13 cpu, 14 device not initialised, 2 launch), -2 out
+ * of memory. m = 0 is allowed: no output rows, and gradients of weights and biases are zero.
+ *
+ * Products are fp32-class: operands carry 22 bits wherever a value is within 2^17 of its tensor's largest, and an
+ * absolute error of 2^-40 of the largest below that; sums are fp32. An infinity or NaN in an operand makes the outputs
+ * that depend on it non-finite, a NaN where fp32 might still have an infinity. Outputs must not overlap inputs, but for
+ * `y` = `residual` exactly.
+ *
+ * The `slb_` calls take their scratch from the pool and give it back before they return, on meta as on cuda, so a dry
+ * run plans it; the `slb_cuda_` calls (cuda only) are given it: 256-byte aligned, at least what the `_scratch_bytes`
+ * call says for these sizes (0 there: sizes refused, or m = 0 and nothing is needed). A scratch buffer serves one call
+ * at a time in stream order. */
+size_t slb_linear_scratch_bytes(int64_t m, int64_t n, int64_t k, int backward);
+size_t slb_gated_scratch_bytes(int64_t m, int64_t f, int64_t k, int backward);
+/* y (m x n) = act(x w^T + bias) + residual for x (m x k), w (n x k); bias and residual may be NULL. The
+ * pre-activations x w^T + bias are kept for the backward pass in `pre` (fp32), in `pre8` (a checkpoint), in both, or
+ * (NULL) not at all. */
+int slb_linear(int dev, const float* x, const float* w, const float* bias, const float* residual, float* y, float* pre,
+               void* pre8, int64_t m, int64_t n, int64_t k, int act);
+int slb_cuda_linear(const float* x, const float* w, const float* bias, const float* residual, float* y, float* pre,
+                    void* pre8, int64_t m, int64_t n, int64_t k, int act, void* scratch, size_t scratch_bytes);
+/* Its gradients: with d = dy * act'(pre), dx = d w, dw = d^T x, db = the column sums of d; each may be NULL, not all.
+ * (The residual's gradient is dy itself.) x and pre are given in fp32 or as checkpoints (x8, pre8), exactly one of each
+ * pair: x for dw, pre when act is not 0; w for dx. */
+int slb_linear_bwd(int dev, const float* dy, const float* x, const void* x8, const float* w, const float* pre,
+                   const void* pre8, float* dx, float* dw, float* db, int64_t m, int64_t n, int64_t k, int act);
+int slb_cuda_linear_bwd(const float* dy, const float* x, const void* x8, const float* w, const float* pre, const void* pre8,
+                        float* dx, float* dw, float* db, int64_t m, int64_t n, int64_t k, int act, void* scratch,
+                        size_t scratch_bytes);
+/* h (m x f) = act(g) * u with g = x wg^T + bg, u = x wu^T + bu; both products, the activation and the product of the two
+ * in one kernel. bg, bu may be NULL. g and u are kept like `pre` above. */
+int slb_gated(int dev, const float* x, const float* wg, const float* wu, const float* bg, const float* bu, float* h, float* g,
+              float* u, void* g8, void* u8, int64_t m, int64_t f, int64_t k, int act);
+int slb_cuda_gated(const float* x, const float* wg, const float* wu, const float* bg, const float* bu, float* h, float* g,
+                   float* u, void* g8, void* u8, int64_t m, int64_t f, int64_t k, int act, void* scratch,
+                   size_t scratch_bytes);
+/* Its gradients: with dg = dh * u * act'(g), du = dh * act(g), dx = dg wg + du wu, dwg = dg^T x, dwu = du^T x, and the
+ * column sums dbg, dbu; each may be NULL, not all. g and u are needed always, each in fp32 or as a checkpoint; x (or x8)
+ * for dwg and dwu; both weights for dx. */
+int slb_gated_bwd(int dev, const float* dh, const float* x, const void* x8, const float* wg, const float* wu, const float* g,
+                  const float* u, const void* g8, const void* u8, float* dx, float* dwg, float* dwu, float* dbg, float* dbu,
+                  int64_t m, int64_t f, int64_t k, int act);
+int slb_cuda_gated_bwd(const float* dh, const float* x, const void* x8, const float* wg, const float* wu, const float* g,
+                       const float* u, const void* g8, const void* u8, float* dx, float* dwg, float* dwu, float* dbg,
+                       float* dbu, int64_t m, int64_t f, int64_t k, int act, void* scratch, size_t scratch_bytes);
+/* A checkpoint of a rows x cols tensor, slb_ck8_bytes(rows, cols) bytes at any alignment: rows * cols signed bytes q,
+ * zero to fifteen unused bytes up to a multiple of 16, then for every row one exponent byte e per 32 columns (the last
+ * group of a row may be shorter). It stands for q * 2^(e - 127). save takes the smallest such step with 127 steps at
+ * least the group's largest magnitude (never below 2^-126) and rounds to nearest, ties to even; a group with an infinity
+ * or a NaN is marked 255 and stands for NaN throughout. load gives the values back; gelu_bwd gives dx = dy * GELU'(x)
+ * for the values x. slb_ck8_bytes gives 0 for sizes that are refused. */
+size_t slb_ck8_bytes(int64_t rows, int64_t cols);
+int slb_ck8_save(int dev, const float* x, void* ck, int64_t rows, int64_t cols);
+int slb_ck8_load(int dev, const void* ck, float* x, int64_t rows, int64_t cols);
+int slb_ck8_gelu_bwd(int dev, const void* ck, const float* dy, float* dx, int64_t rows, int64_t cols);
 /* Test hook: `world` ranks emulated on one GPU by one cooperative launch (blocks of all ranks resident together).
  * Pointer arrays are indexed [rank * nseg + segment]; p/m/v may be NULL when adam = 0. mode: 0 auto, 1 one-shot,
  * 2 two-shot. active_mask: bit r set = rank r takes part (a missing rank makes the others' waits run out).

@@ -147,6 +147,11 @@ public:
     void copy_blocking(void* dst, const void* src, size_t n, int kind);
     // Memory is about to go back to the allocator: the legacy stream waits for lane work that still uses it.
     void before_release(const void* p, size_t n);
+    // For operators that launch on the legacy stream themselves: it waits for lane work that conflicts with this
+    // memory; afterwards the launches are counted, and lanes wait for them.
+    void legacy_touches(const void* p, size_t n, bool write) { lanes_.legacy_touches(p, n, write); }
+    void legacy_launches(int n) { launches += (uint64_t)n, legacy_epoch_++; }
+    int* status_word() const { return status_dev_; }  // device address of this rank's sticky status, or null
 
     // --- copies beside the path (pinned host memory), k buffers per call; 0 or -1
     int from_host_async(int k, void* const* dst, const void* const* src, const size_t* bytes);

@@ -91,6 +91,7 @@ enum Status : int {
     ST_TIMEOUT_START = 21,   // a peer never announced its gradients
     ST_TIMEOUT_REDUCED = 22, // a peer never announced its reduced chunk / its staged gradients
     ST_TIMEOUT_DONE = 23,    // a peer never announced that it finished reading
+    ST_TIMEOUT_PRODUCT = 24, // a wait inside a matrix product ran out
 };
 
 struct LaunchArgs {
@@ -114,7 +115,7 @@ enum Err : int {
     ERR_BAD_ARG = 12,        // misuse of an entry point (null/odd pointer, negative size, too many segments)
     ERR_NO_CPU_COMPUTE = 13, // a compute op was asked to run on the cpu device: this library has no host kernels
     ERR_NO_WORKSPACE = 14,   // the device was not initialised through sl_init_device
-    ERR_PEER = 20,           // 21..23: a bounded wait on a peer ran out (see Status)
+    ERR_PEER = 20,           // 21..24: a bounded wait on the device ran out (see Status)
 };
 
 }  // namespace slb

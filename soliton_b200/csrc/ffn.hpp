@@ -1,0 +1,150 @@
+// What the feed-forward operators (ffn_api.cu) hand to their kernels: operand planes (ffn_pack.cu), matrix products
+// over them (ffn_gemm.cu) and 8-bit activation checkpoints (ck8_kernels.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace slb_ffn {
+
+enum Act : int { ACT_NONE = 0, ACT_GELU = 1, ACT_SILU = 2 };
+
+// ---------------------------------------------------------------- operand planes
+//
+// A plane holds a rows x cols matrix as fp16 pieces in blocks of 64 x 64. A block is the image of its values in shared
+// memory as the tensor cores read it: row r at byte 128 r, the row's eight 16-byte chunks at positions c ^ (r & 7) (the
+// 128-byte swizzle). The same image serves as 64 rows of a K-major operand tile and as 64 columns of an MN-major one, so
+// one plane feeds every product its matrix appears in, transposed or not. A block is `pieces` images of 8 KiB: the
+// value's upper 11 bits and, in a plane of two, the 11 bits that follow. Rows and columns beyond the matrix are zero.
+constexpr int kBlock = 64;
+constexpr size_t kImageBytes = kBlock * kBlock * 2;
+constexpr int kAmaxParts = 296;     // partial maxima per tensor at the most, one per block of the maximum's kernel
+constexpr int kMaxSlots = 6;        // tensors whose maxima one call needs
+constexpr int kMaxJobs = 4;
+constexpr int kMaxPlanes = 3;
+
+// One tensor whose largest finite magnitude is wanted, as an exponent: fp32 values, or the exponent bytes of a checkpoint.
+struct AmaxSlot {
+    const void* p;
+    int64_t n;
+    int is_ck8;
+    int parts;                      // partial maxima, at most kAmaxParts
+};
+struct AmaxArgs {
+    AmaxSlot slot[kMaxSlots];
+    int slots;
+    float* parts;                   // kMaxSlots x kAmaxParts
+};
+
+enum PackKind : int {
+    PACK_FP32 = 0,      // the matrix itself
+    PACK_CK8 = 1,       // a checkpoint: one piece holds its values exactly
+    PACK_ACT = 2,       // dy * act'(pre), pre in fp32 or a checkpoint
+    PACK_GATED = 3,     // dh * u * act'(g) and, into the second half of the plane, dh * act(g)
+};
+struct PackJob {
+    int kind, act;
+    const float* a;                 // the matrix, dy or dh
+    const float *b, *c;             // pre, or g and u, in fp32 ...
+    const void *b8, *c8;            // ... or as checkpoints; `b8` alone with PACK_CK8
+    int64_t rows, cols;
+    int row_blocks, col_blocks;     // of this matrix
+    int row_stride;                 // blocks per block row of the plane
+    int second;                     // PACK_GATED: blocks from a value's block to its partner's
+    int pieces;
+    char* plane;                    // the matrix's first block
+    float* colsum;                  // null, or row_blocks x cols floats: the column sums of each block row
+    float* colsum2;                 // the same for PACK_GATED's second matrix
+    int slots;                      // bit s: maximum s bounds this job's values (PACK_FP32, PACK_CK8)
+    int plane_id;                   // which exponent of `exps` is this plane's
+    int first_unit;                 // blocks of the jobs before this one
+};
+struct PackArgs {
+    PackJob job[kMaxJobs];
+    int jobs, units;
+    AmaxArgs amax;
+    int* exps;                      // out: values of plane i were multiplied by 2^(15 - exps[i])
+};
+
+// ---------------------------------------------------------------- products
+
+// Operand: blocks of a plane addressed by (index along M or N, index along K).
+struct Operand {
+    const char* plane;
+    int64_t mn_stride, k_stride;    // in blocks
+    int mn_blocks;                  // blocks along M or N that exist
+    int exp_id;
+};
+enum Epilogue : int { EPI_STORE = 0, EPI_LINEAR = 1, EPI_GATED = 2 };
+struct GemmArgs {
+    Operand a, b;
+    int k_blocks;
+    int m_tiles, n_tiles;
+    const int* exps;
+    int* status;                    // sticky status word (host memory), or null
+    unsigned long long timeout_ns;  // bound of every wait
+    int64_t rows, cols;             // of the output (EPI_GATED: cols of each of the two)
+    int64_t split;                  // EPI_STORE: output rows from here on (a multiple of 64) go to out2, counted from 0
+    float *out, *out2;
+    int act;
+    const float *bias, *bias2, *residual;
+    float *save, *save2;            // pre-activations in fp32 ...
+    char *save8, *save8_2;          // ... or as checkpoints
+    int gate_blocks;                // EPI_GATED: blocks of the gate's weight; the second weight's follow in the plane
+};
+
+cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
+cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st);
+// out[j] = the sum over `parts` of the block rows' column sums, in order
+cudaError_t launch_colsum(const float* parts, int count, int64_t cols, float* out, cudaStream_t st);
+// a_mn, b_mn: the operand's blocks hold K along their rows. pieces_b: 1 when B is a checkpoint's plane.
+cudaError_t launch_gemm(const GemmArgs& g, bool a_mn, bool b_mn, int pieces_b, Epilogue epi, int sm_count, cudaStream_t st);
+
+// ---------------------------------------------------------------- checkpoints in 8 bits
+
+constexpr int kGroup = 32;
+inline __host__ __device__ int64_t ck8_groups(int64_t cols) { return (cols + kGroup - 1) / kGroup; }
+inline __host__ __device__ int64_t ck8_exp_offset(int64_t rows, int64_t cols) { return (rows * cols + 15) / 16 * 16; }
+inline __host__ __device__ int64_t ck8_bytes(int64_t rows, int64_t cols) {
+    return ck8_exp_offset(rows, cols) + rows * ck8_groups(cols);
+}
+cudaError_t launch_ck8_save(const float* x, char* ck, int64_t rows, int64_t cols, int sm_count, cudaStream_t st);
+cudaError_t launch_ck8_load(const char* ck, float* x, int64_t rows, int64_t cols, int sm_count, cudaStream_t st);
+cudaError_t launch_ck8_gelu_bwd(const char* ck, const float* dy, float* dx, int64_t rows, int64_t cols, int sm_count, cudaStream_t st);
+
+#ifdef __CUDACC__
+// The exponent byte of a group whose largest magnitude has these bits (sign cleared): the smallest e >= -126 with
+// 127 * 2^e >= the magnitude, plus 127; 255 when the group holds an infinity or a NaN. In a normal magnitude
+// 1.f * 2^p, 127 * 2^(p - 6) = 1.984375 * 2^p suffices up to f = 0.984375 and 2^(p - 5) is needed beyond.
+__device__ __forceinline__ unsigned ck8_exponent(unsigned bits) {
+    if (bits >= 0x7f800000u) return 255u;
+    const int p = (int)(bits >> 23) - 127;
+    const int e = p - 6 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    return (unsigned)((e < -126 ? -126 : e) + 127);
+}
+// 2^(byte - 127) for bytes 1..254; a byte of 0 stands for 2^-127; 255 gives NaN.
+__device__ __forceinline__ float ck8_step(unsigned byte) {
+    return byte == 255u ? __int_as_float(0x7fc00000) : byte == 0u ? __int_as_float(0x00400000) : __int_as_float((int)(byte << 23));
+}
+// The reciprocal step, a power of two as well: bytes that ck8_exponent gives are 1..249, so 254 - byte is 5..253.
+__device__ __forceinline__ float ck8_inv_step(unsigned byte) { return byte == 255u ? 0.0f : __int_as_float((int)((254u - byte) << 23)); }
+// Nearest multiple of the step, ties to even; |x| <= 127 steps by the choice of the exponent. Groups marked 255 store 0.
+__device__ __forceinline__ int ck8_quantise(float x, float inv_step, unsigned byte) { return byte == 255u ? 0 : __float2int_rn(x * inv_step); }
+
+__device__ __forceinline__ float act_of(int act, float v) {
+    if (act == ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    if (act == ACT_SILU) return v / (1.0f + expf(-v));
+    return v;
+}
+__device__ __forceinline__ float act_grad(int act, float v) {
+    if (act == ACT_GELU) return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * (expf(-0.5f * v * v) * 0.39894228f);
+    if (act == ACT_SILU) {
+        const float sig = 1.0f / (1.0f + expf(-v));
+        return sig * (1.0f + v * (1.0f - sig));
+    }
+    return 1.0f;
+}
+#endif
+
+}  // namespace slb_ffn

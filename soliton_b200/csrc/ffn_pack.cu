@@ -1,0 +1,273 @@
+// Operand planes for the products (ffn.hpp): the largest magnitude of each tensor, then fp32 values (or a checkpoint's,
+// or the gradient that an activation hands back) as scaled fp16 pieces in the tensor cores' block layout.
+//
+// The tensor cores have no fp32. A value times a power of two, t = x * 2^(15 - E) with |x| < 2^E for the whole tensor,
+// is cut into hi = fp16(t) and lo = fp16(t - hi): 22 bits of x wherever |x| > 2^(E - 17), and an absolute error of
+// 2^(E - 40) below that. A product of two such values takes three fp16 products, hi*hi + hi*lo + lo*hi; the dropped
+// lo*lo is below 2^-22 of it. TF32 pieces would need three products too, at half the rate; bf16 pieces six for the
+// same bits. The price is E, known only after the whole tensor has been seen: one more read of the tensor, which
+// leaves it in L2 for the second. A bound serves as well as the maximum (17 binades of full precision are far more than
+// needed), so dy * act'(pre) is bounded from dy alone and the gated gradients from the three tensors' own maxima.
+// Infinities and NaN do not count towards a maximum; as operands they become infinities and NaN.
+//
+// Bound by HBM: 4 B read for the maximum, 4 B read and 4 B written per value for the plane.
+#include <cuda_fp16.h>
+
+#include "ffn.hpp"
+
+namespace slb_ffn {
+
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------- maxima
+
+// Maxima of magnitudes as bit patterns: for finite floats they order as the values do.
+__device__ __forceinline__ unsigned finite_bits(float x) {
+    const unsigned b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ unsigned finite_byte(unsigned byte) { return byte == 255u ? 0u : byte; }
+
+__global__ void __launch_bounds__(kThreads) k_amax(AmaxArgs a) {
+    const int s = blockIdx.y;
+    const AmaxSlot t = a.slot[s];
+    if ((int)blockIdx.x >= t.parts) return;
+    unsigned top = 0;
+    const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, step = (int64_t)t.parts * kThreads;
+    if (t.is_ck8) {
+        const unsigned char* p = static_cast<const unsigned char*>(t.p);
+        for (int64_t i = at; i < t.n; i += step) top = max(top, finite_byte(p[i]));
+    } else {
+        const float* p = static_cast<const float*>(t.p);
+        // up to three values ahead of the first 16-byte boundary, then 128-bit words, then the rest
+        int64_t head = (int64_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / 4;
+        if (head > t.n) head = t.n;
+        const int64_t words = (t.n - head) / 4;
+        const float4* w = reinterpret_cast<const float4*>(p + head);
+        int64_t i = at;
+        for (; i + 3 * step < words; i += 4 * step) {
+            float4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = __ldg(w + i + u * step);
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                top = max(max(top, max(finite_bits(v[u].x), finite_bits(v[u].y))), max(finite_bits(v[u].z), finite_bits(v[u].w)));
+        }
+        for (; i < words; i += step) {
+            const float4 v = __ldg(w + i);
+            top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+        }
+        if (at < head) top = max(top, finite_bits(p[at]));
+        if (at < t.n - head - 4 * words) top = max(top, finite_bits(p[head + 4 * words + at]));
+    }
+    __shared__ unsigned part[kThreads / 32];
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        top = __reduce_max_sync(0xffffffffu, threadIdx.x < kThreads / 32 ? part[threadIdx.x] : 0u);
+        if (threadIdx.x == 0) a.parts[s * kAmaxParts + blockIdx.x] = __uint_as_float(top);
+    }
+}
+
+// E with every finite |x| < 2^E: from the largest magnitude's bits, or the largest exponent byte (|q| <= 127 < 2^7).
+__device__ __forceinline__ int exponent_of(unsigned top, int is_ck8) {
+    if (is_ck8) return (int)top - 127 + 7;
+    return (int)(top >> 23) - 126;
+}
+constexpr int kLeastExp = -110, kMostExp = 128;  // so that 2^(15 - E) and its reciprocal are normal floats
+
+// ---------------------------------------------------------------- planes
+
+struct Eight {
+    float v[8];
+};
+// Eight values from p on, of which `have` exist; `wide`: 16-byte loads may be used.
+__device__ __forceinline__ Eight load8(const float* p, int have, bool wide) {
+    Eight r;
+    if (wide && have == 8) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(p)), y = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        r.v[0] = x.x, r.v[1] = x.y, r.v[2] = x.z, r.v[3] = x.w, r.v[4] = y.x, r.v[5] = y.y, r.v[6] = y.z, r.v[7] = y.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.v[i] = i < have ? __ldg(p + i) : 0.0f;
+    }
+    return r;
+}
+// The same from a checkpoint: eight columns from a multiple of eight lie in one group.
+__device__ __forceinline__ Eight load8_ck(const void* ck, int64_t rows, int64_t cols, int64_t row, int64_t col, int have, bool wide) {
+    const signed char* q = static_cast<const signed char*>(ck) + row * cols + col;
+    const unsigned char* e = static_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols) + row * ck8_groups(cols) + col / kGroup;
+    const float step = ck8_step(__ldg(e));
+    Eight r;
+    if (wide && have == 8) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            r.v[i] = (float)(signed char)(w.x >> (8 * i)) * step;
+            r.v[4 + i] = (float)(signed char)(w.y >> (8 * i)) * step;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.v[i] = i < have ? (float)__ldg(q + i) * step : 0.0f;
+    }
+    return r;
+}
+
+__device__ __forceinline__ void split8(const Eight& x, float scale, uint4& hi, uint4& lo) {
+    unsigned h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float a = x.v[2 * i] * scale, b = x.v[2 * i + 1] * scale;
+        const __half2 p = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(p);
+        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+        h[i] = *reinterpret_cast<const unsigned*>(&p), l[i] = *reinterpret_cast<const unsigned*>(&r);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]), lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+__device__ __forceinline__ void store_pieces(char* block, int pieces, int at, const Eight& x, float scale) {
+    uint4 hi, lo;
+    split8(x, scale, hi, lo);
+    *reinterpret_cast<uint4*>(block + at) = hi;
+    if (pieces == 2) *reinterpret_cast<uint4*>(block + kImageBytes + at) = lo;
+}
+
+// Column sums over a block's 64 rows: a thread holds two rows' eight columns; four rows meet in a warp, then the eight
+// warps in order.
+__device__ __forceinline__ void block_colsum(const Eight (&x)[2], float (&buf)[8][kBlock], float* out, int64_t col0, int64_t cols) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        t[i] = x[0].v[i] + x[1].v[i];
+        t[i] += __shfl_xor_sync(0xffffffffu, t[i], 8);
+        t[i] += __shfl_xor_sync(0xffffffffu, t[i], 16);
+    }
+    __syncthreads();  // whoever read `buf` last is done
+    if (lane < 8)
+#pragma unroll
+        for (int i = 0; i < 8; i++) buf[warp][lane * 8 + i] = t[i];
+    __syncthreads();
+    if (threadIdx.x < kBlock && col0 + threadIdx.x < cols) {
+        float sum = buf[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 8; w++) sum += buf[w][threadIdx.x];
+        out[col0 + threadIdx.x] = sum;
+    }
+}
+
+// A block of threads takes blocks of 64 x 64 round robin over all jobs; a thread eight columns of two rows.
+__global__ void __launch_bounds__(kThreads) k_pack(const __grid_constant__ PackArgs a) {
+    __shared__ int s_exp[kMaxSlots];
+    __shared__ float s_sum[8][kBlock];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < a.amax.slots) {
+        unsigned top = 0;
+        for (int i = lane; i < a.amax.slot[warp].parts; i += 32) top = max(top, __float_as_uint(a.amax.parts[warp * kAmaxParts + i]));
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) s_exp[warp] = exponent_of(top, a.amax.slot[warp].is_ck8);
+    }
+    __syncthreads();
+    const int chunk = threadIdx.x & 7, row_in = threadIdx.x >> 3;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        int ji = 0;
+        while (ji + 1 < a.jobs && unit >= a.job[ji + 1].first_unit) ji++;
+        const PackJob& j = a.job[ji];
+        int e;
+        if (j.kind == PACK_GATED) {
+            e = s_exp[0] + max(s_exp[1] + (j.act != ACT_NONE), s_exp[2]);  // |act'| < 2, |act(g)| <= |g|
+        } else if (j.kind == PACK_ACT) {
+            e = s_exp[0] + 1;
+        } else {
+            e = kLeastExp;
+            for (int s = 0; s < a.amax.slots; s++)
+                if (j.slots >> s & 1) e = max(e, s_exp[s]);
+        }
+        e = min(max(e, kLeastExp), kMostExp);
+        if (unit == j.first_unit && threadIdx.x == 0) a.exps[j.plane_id] = e;
+        const float scale = exp2f((float)(15 - e));
+        const int u = unit - j.first_unit, rb = u / j.col_blocks, cb = u - rb * j.col_blocks;
+        const int64_t col = (int64_t)cb * kBlock + chunk * 8;
+        const int have = col >= j.cols ? 0 : j.cols - col < 8 ? (int)(j.cols - col) : 8;
+        const bool wide = (j.cols & 7) == 0;
+        char* block = j.plane + ((int64_t)rb * j.row_stride + cb) * (int64_t)(j.pieces * kImageBytes);
+        Eight x[2], y[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = row_in + 32 * h;
+            const int64_t row = (int64_t)rb * kBlock + r;
+            const int got = row < j.rows ? have : 0;
+            const int64_t off = row * j.cols + col;
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[h].v[i] = 0.0f, y[h].v[i] = 0.0f;
+            if (got > 0) {
+                if (j.kind == PACK_CK8) {
+                    x[h] = load8_ck(j.b8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.b8) & 7) == 0);
+                } else {
+                    x[h] = load8(j.a + off, got, wide && (reinterpret_cast<uintptr_t>(j.a) & 15) == 0);
+                    if (j.kind == PACK_ACT) {
+                        const Eight pre = j.b8 ? load8_ck(j.b8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.b8) & 7) == 0)
+                                               : load8(j.b + off, got, wide && (reinterpret_cast<uintptr_t>(j.b) & 15) == 0);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[h].v[i] *= act_grad(j.act, pre.v[i]);
+                    } else if (j.kind == PACK_GATED) {
+                        const Eight g = j.b8 ? load8_ck(j.b8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.b8) & 7) == 0)
+                                             : load8(j.b + off, got, wide && (reinterpret_cast<uintptr_t>(j.b) & 15) == 0);
+                        const Eight up = j.c8 ? load8_ck(j.c8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.c8) & 7) == 0)
+                                              : load8(j.c + off, got, wide && (reinterpret_cast<uintptr_t>(j.c) & 15) == 0);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float d = x[h].v[i];
+                            x[h].v[i] = d * up.v[i] * act_grad(j.act, g.v[i]);
+                            y[h].v[i] = d * act_of(j.act, g.v[i]);
+                        }
+                    }
+                }
+            }
+            const int at = r * 128 + ((chunk ^ (r & 7)) << 4);
+            store_pieces(block, j.pieces, at, x[h], scale);
+            if (j.kind == PACK_GATED) store_pieces(block + (int64_t)j.second * (int64_t)(j.pieces * kImageBytes), j.pieces, at, y[h], scale);
+        }
+        if (j.colsum) block_colsum(x, s_sum, j.colsum + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+        if (j.colsum2) block_colsum(y, s_sum, j.colsum2 + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+    }
+}
+
+// A thread per column, block rows in order, eight loads in flight.
+__global__ void __launch_bounds__(kThreads) k_colsum(const float* __restrict__ parts, int count, int64_t cols, float* __restrict__ out) {
+    const int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (j >= cols) return;
+    float sum = 0;
+    int i = 0;
+    for (; i + 8 <= count; i += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = parts[(int64_t)(i + u) * cols + j];
+#pragma unroll
+        for (int u = 0; u < 8; u++) sum += v[u];
+    }
+    for (; i < count; i++) sum += parts[(int64_t)i * cols + j];
+    out[j] = sum;
+}
+
+cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {
+    int most = 1;
+    for (int s = 0; s < a.slots; s++) most = most > a.slot[s].parts ? most : a.slot[s].parts;
+    k_amax<<<dim3((unsigned)most, (unsigned)a.slots), kThreads, 0, st>>>(a);
+    return cudaPeekAtLastError();
+}
+
+cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st) {
+    const int most = sm_count * 8;
+    k_pack<<<a.units < most ? a.units : most, kThreads, 0, st>>>(a);
+    return cudaPeekAtLastError();
+}
+
+cudaError_t launch_colsum(const float* parts, int count, int64_t cols, float* out, cudaStream_t st) {
+    k_colsum<<<(unsigned)((cols + kThreads - 1) / kThreads), kThreads, 0, st>>>(parts, count, cols, out);
+    return cudaPeekAtLastError();
+}
+
+}  // namespace slb_ffn
