@@ -80,7 +80,7 @@ enum Epilogue : int { EPI_STORE = 0, EPI_LINEAR = 1, EPI_GATED = 2 };
 struct GemmArgs {
     Operand a, b;
     int k_blocks;
-    int m_tiles, n_tiles;
+    int m_tiles, n_tiles;           // set by launch_gemm
     const int* exps;
     int* status;                    // sticky status word (host memory), or null
     unsigned long long timeout_ns;  // bound of every wait
@@ -92,6 +92,7 @@ struct GemmArgs {
     float *save, *save2;            // pre-activations in fp32 ...
     char *save8, *save8_2;          // ... or as checkpoints
     int gate_blocks;                // EPI_GATED: blocks of the gate's weight; the second weight's follow in the plane
+    int wide;                       // set by launch_gemm: rows and pointers allow 16-byte accesses (4-byte for checkpoints)
 };
 
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
@@ -132,16 +133,29 @@ __device__ __forceinline__ float ck8_inv_step(unsigned byte) { return byte == 25
 // Nearest multiple of the step, ties to even; |x| <= 127 steps by the choice of the exponent. Groups marked 255 store 0.
 __device__ __forceinline__ int ck8_quantise(float x, float inv_step, unsigned byte) { return byte == 255u ? 0 : __float2int_rn(x * inv_step); }
 
+// Two ulps at most each, as CUDA documents them; what an argument's rounding adds is relative to terms that vanish with it.
+__device__ __forceinline__ float fast_exp(float v) { return __expf(v); }
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + fast_exp(-v)); }
+
 __device__ __forceinline__ float act_of(int act, float v) {
     if (act == ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    if (act == ACT_SILU) return v / (1.0f + expf(-v));
+    if (act == ACT_SILU) return v * sigmoid(v);
     return v;
 }
+// GELU' = Phi(v) + v phi(v). Both share exp(-v^2 / 2): 1 - erf(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), for z >= 0
+// (Abramowitz and Stegun 7.1.26), off by 1.5e-7 at most, which Phi halves: about an ulp of a derivative near one, at under
+// half the instructions of erff and expf apart.
 __device__ __forceinline__ float act_grad(int act, float v) {
-    if (act == ACT_GELU) return 0.5f * (1.0f + erff(v * 0.70710678f)) + v * (expf(-0.5f * v * v) * 0.39894228f);
+    if (act == ACT_GELU) {
+        const float z = fabsf(v) * 0.70710678f, e = fast_exp(-0.5f * v * v);
+        const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
+        const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        const float tail = 0.5f * poly * e;                     // Phi(-|v|)
+        return fmaf(v * 0.39894228f, e, v < 0.0f ? tail : 1.0f - tail);
+    }
     if (act == ACT_SILU) {
-        const float sig = 1.0f / (1.0f + expf(-v));
-        return sig * (1.0f + v * (1.0f - sig));
+        const float sig = sigmoid(v);
+        return sig * fmaf(v, 1.0f - sig, 1.0f);
     }
     return 1.0f;
 }

@@ -18,6 +18,7 @@
 namespace slb_ffn {
 
 constexpr int kThreads = 256;
+constexpr int kPackPerSM = 3;       // blocks of k_pack on one SM: 80 registers a thread hold two rows of three tensors
 
 // ---------------------------------------------------------------- maxima
 
@@ -158,8 +159,52 @@ __device__ __forceinline__ void block_colsum(const Eight (&x)[2], float (&buf)[8
     }
 }
 
-// A block of threads takes blocks of 64 x 64 round robin over all jobs; a thread eight columns of two rows.
-__global__ void __launch_bounds__(kThreads) k_pack(const __grid_constant__ PackArgs a) {
+// Eight columns of `row` of a job's operand, in fp32 or from its checkpoint.
+__device__ __forceinline__ Eight load8_held(const PackJob& j, const float* p, const void* ck, int64_t row, int64_t col, int have) {
+    if (have == 0) return load8(nullptr, 0, false);
+    const bool whole = (j.cols & 7) == 0;
+    return ck ? load8_ck(ck, j.rows, j.cols, row, col, have, whole && (reinterpret_cast<uintptr_t>(ck) & 7) == 0)
+              : load8(p + row * j.cols + col, have, whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0);
+}
+
+// One block of 64 x 64: a thread takes eight columns of two rows, all of whose loads are issued before the first is used.
+template <int KIND>
+__device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scale, float (&s_sum)[8][kBlock]) {
+    const int chunk = threadIdx.x & 7, row_in = threadIdx.x >> 3;
+    const int u = unit - j.first_unit, rb = u / j.col_blocks, cb = u - rb * j.col_blocks;
+    const int64_t col = (int64_t)cb * kBlock + chunk * 8;
+    const int have = col >= j.cols ? 0 : j.cols - col < 8 ? (int)(j.cols - col) : 8;
+    char* block = j.plane + ((int64_t)rb * j.row_stride + cb) * (int64_t)(j.pieces * kImageBytes);
+    Eight x[2], y[2], z[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int64_t row = (int64_t)rb * kBlock + row_in + 32 * h;
+        const int got = row < j.rows ? have : 0;
+        x[h] = load8_held(j, j.a, KIND == PACK_CK8 ? j.b8 : nullptr, row, col, got);
+        if (KIND == PACK_ACT || KIND == PACK_GATED) y[h] = load8_held(j, j.b, j.b8, row, col, got);
+        if (KIND == PACK_GATED) z[h] = load8_held(j, j.c, j.c8, row, col, got);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = row_in + 32 * h, at = r * 128 + ((chunk ^ (r & 7)) << 4);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (KIND == PACK_ACT) x[h].v[i] *= act_grad(j.act, y[h].v[i]);
+            if (KIND == PACK_GATED) {
+                const float d = x[h].v[i], gate = y[h].v[i];
+                x[h].v[i] = d * z[h].v[i] * act_grad(j.act, gate);
+                y[h].v[i] = d * act_of(j.act, gate);
+            }
+        }
+        store_pieces(block, KIND == PACK_CK8 ? 1 : 2, at, x[h], scale);
+        if (KIND == PACK_GATED) store_pieces(block + (int64_t)j.second * (int64_t)(2 * kImageBytes), 2, at, y[h], scale);
+    }
+    if (KIND != PACK_CK8 && j.colsum) block_colsum(x, s_sum, j.colsum + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+    if (KIND == PACK_GATED && j.colsum2) block_colsum(y, s_sum, j.colsum2 + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+}
+
+// Blocks of threads take blocks of 64 x 64 round robin over all jobs.
+__global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_constant__ PackArgs a) {
     __shared__ int s_exp[kMaxSlots];
     __shared__ float s_sum[8][kBlock];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -170,9 +215,8 @@ __global__ void __launch_bounds__(kThreads) k_pack(const __grid_constant__ PackA
         if (lane == 0) s_exp[warp] = exponent_of(top, a.amax.slot[warp].is_ck8);
     }
     __syncthreads();
-    const int chunk = threadIdx.x & 7, row_in = threadIdx.x >> 3;
+    int ji = 0;
     for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        int ji = 0;
         while (ji + 1 < a.jobs && unit >= a.job[ji + 1].first_unit) ji++;
         const PackJob& j = a.job[ji];
         int e;
@@ -188,68 +232,31 @@ __global__ void __launch_bounds__(kThreads) k_pack(const __grid_constant__ PackA
         e = min(max(e, kLeastExp), kMostExp);
         if (unit == j.first_unit && threadIdx.x == 0) a.exps[j.plane_id] = e;
         const float scale = exp2f((float)(15 - e));
-        const int u = unit - j.first_unit, rb = u / j.col_blocks, cb = u - rb * j.col_blocks;
-        const int64_t col = (int64_t)cb * kBlock + chunk * 8;
-        const int have = col >= j.cols ? 0 : j.cols - col < 8 ? (int)(j.cols - col) : 8;
-        const bool wide = (j.cols & 7) == 0;
-        char* block = j.plane + ((int64_t)rb * j.row_stride + cb) * (int64_t)(j.pieces * kImageBytes);
-        Eight x[2], y[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = row_in + 32 * h;
-            const int64_t row = (int64_t)rb * kBlock + r;
-            const int got = row < j.rows ? have : 0;
-            const int64_t off = row * j.cols + col;
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[h].v[i] = 0.0f, y[h].v[i] = 0.0f;
-            if (got > 0) {
-                if (j.kind == PACK_CK8) {
-                    x[h] = load8_ck(j.b8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.b8) & 7) == 0);
-                } else {
-                    x[h] = load8(j.a + off, got, wide && (reinterpret_cast<uintptr_t>(j.a) & 15) == 0);
-                    if (j.kind == PACK_ACT) {
-                        const Eight pre = j.b8 ? load8_ck(j.b8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.b8) & 7) == 0)
-                                               : load8(j.b + off, got, wide && (reinterpret_cast<uintptr_t>(j.b) & 15) == 0);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) x[h].v[i] *= act_grad(j.act, pre.v[i]);
-                    } else if (j.kind == PACK_GATED) {
-                        const Eight g = j.b8 ? load8_ck(j.b8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.b8) & 7) == 0)
-                                             : load8(j.b + off, got, wide && (reinterpret_cast<uintptr_t>(j.b) & 15) == 0);
-                        const Eight up = j.c8 ? load8_ck(j.c8, j.rows, j.cols, row, col, got, wide && (reinterpret_cast<uintptr_t>(j.c8) & 7) == 0)
-                                              : load8(j.c + off, got, wide && (reinterpret_cast<uintptr_t>(j.c) & 15) == 0);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float d = x[h].v[i];
-                            x[h].v[i] = d * up.v[i] * act_grad(j.act, g.v[i]);
-                            y[h].v[i] = d * act_of(j.act, g.v[i]);
-                        }
-                    }
-                }
-            }
-            const int at = r * 128 + ((chunk ^ (r & 7)) << 4);
-            store_pieces(block, j.pieces, at, x[h], scale);
-            if (j.kind == PACK_GATED) store_pieces(block + (int64_t)j.second * (int64_t)(j.pieces * kImageBytes), j.pieces, at, y[h], scale);
-        }
-        if (j.colsum) block_colsum(x, s_sum, j.colsum + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
-        if (j.colsum2) block_colsum(y, s_sum, j.colsum2 + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+        if (j.kind == PACK_FP32) pack_unit<PACK_FP32>(j, unit, scale, s_sum);
+        else if (j.kind == PACK_CK8) pack_unit<PACK_CK8>(j, unit, scale, s_sum);
+        else if (j.kind == PACK_ACT) pack_unit<PACK_ACT>(j, unit, scale, s_sum);
+        else pack_unit<PACK_GATED>(j, unit, scale, s_sum);
     }
 }
 
-// A thread per column, block rows in order, eight loads in flight.
+// A block takes 32 columns, each of its warps every eighth block row; the eight sums meet in order.
 __global__ void __launch_bounds__(kThreads) k_colsum(const float* __restrict__ parts, int count, int64_t cols, float* __restrict__ out) {
-    const int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (j >= cols) return;
+    __shared__ float part[kThreads / 32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t j = (int64_t)blockIdx.x * 32 + lane;
     float sum = 0;
-    int i = 0;
-    for (; i + 8 <= count; i += 8) {
-        float v[8];
-#pragma unroll
-        for (int u = 0; u < 8; u++) v[u] = parts[(int64_t)(i + u) * cols + j];
-#pragma unroll
-        for (int u = 0; u < 8; u++) sum += v[u];
+    if (j < cols) {
+#pragma unroll 8
+        for (int i = warp; i < count; i += kThreads / 32) sum += parts[(int64_t)i * cols + j];
     }
-    for (; i < count; i++) sum += parts[(int64_t)i * cols + j];
-    out[j] = sum;
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && j < cols) {
+        sum = part[0][lane];
+#pragma unroll
+        for (int w = 1; w < kThreads / 32; w++) sum += part[w][lane];
+        out[j] = sum;
+    }
 }
 
 cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {
@@ -260,13 +267,13 @@ cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {
 }
 
 cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st) {
-    const int most = sm_count * 8;
+    const int most = sm_count * kPackPerSM;  // as many as run at once: each starts with the maxima
     k_pack<<<a.units < most ? a.units : most, kThreads, 0, st>>>(a);
     return cudaPeekAtLastError();
 }
 
 cudaError_t launch_colsum(const float* parts, int count, int64_t cols, float* out, cudaStream_t st) {
-    k_colsum<<<(unsigned)((cols + kThreads - 1) / kThreads), kThreads, 0, st>>>(parts, count, cols, out);
+    k_colsum<<<(unsigned)((cols + 31) / 32), kThreads, 0, st>>>(parts, count, cols, out);
     return cudaPeekAtLastError();
 }
 
