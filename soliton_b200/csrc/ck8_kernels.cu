@@ -13,50 +13,143 @@ namespace slb_ffn {
 
 constexpr int kThreads = 256;
 
-// A warp per group of 32 columns, a lane per column.
-__global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__ x, char* __restrict__ ck, int64_t rows, int64_t cols) {
+// Columns a multiple of 32 and aligned buffers: rows run on without a break in groups, so the tensor is one long row of
+// groups. A lane holds four columns, eight lanes a group; a thread has four such quarters of a group in flight, a block's
+// threads side by side in each.
+constexpr int kAhead = 4;
+
+__global__ void __launch_bounds__(kThreads) k_ck8_save_wide(const float4* __restrict__ x, unsigned* __restrict__ q, unsigned char* __restrict__ eb,
+                                                            int64_t quads) {
     const int lane = threadIdx.x & 31;
-    const int64_t groups = ck8_groups(cols), total = rows * groups, step = (int64_t)gridDim.x * (kThreads / 32);
-    unsigned char* eb = reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols);
-    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < total; i += step) {
-        const int64_t row = i / groups, col = (i - row * groups) * kGroup + lane;
-        const float v = col < cols ? x[row * cols + col] : 0.0f;
-        const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
-        if (col < cols) ck[row * cols + col] = (char)ck8_quantise(v, ck8_inv_step(byte), byte);
-        if (lane == 0) eb[i] = (unsigned char)byte;
+    const int64_t first = (int64_t)blockIdx.x * (kThreads * kAhead) + threadIdx.x;
+    float4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+        if (first + i * kThreads < quads) v[i] = __ldcs(x + first + i * kThreads);
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        const int64_t at = first + i * kThreads;
+        if (at >= quads) break;  // quads is a multiple of eight: the eight lanes of a group leave together
+        unsigned top = max(max(__float_as_uint(v[i].x) & 0x7fffffffu, __float_as_uint(v[i].y) & 0x7fffffffu),
+                           max(__float_as_uint(v[i].z) & 0x7fffffffu, __float_as_uint(v[i].w) & 0x7fffffffu));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffu << (lane & 24), top, o));
+        const unsigned byte = ck8_exponent(top);
+        q[at] = ck8_quantise4(v[i].x, v[i].y, v[i].z, v[i].w, byte);
+        if ((lane & 7) == 0) eb[at >> 3] = (unsigned char)byte;
     }
 }
 
 template <bool GELU_BWD>
-__global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ ck, const float* __restrict__ dy, float* __restrict__ out,
-                                                       int64_t rows, int64_t cols) {
-    const int lane = threadIdx.x & 31;
-    const int64_t groups = ck8_groups(cols), total = rows * groups, step = (int64_t)gridDim.x * (kThreads / 32);
-    const unsigned char* eb = reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols);
-    for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < total; i += step) {
-        const int64_t row = i / groups, col = (i - row * groups) * kGroup + lane;
-        if (col >= cols) continue;
-        const float v = (float)(signed char)ck[row * cols + col] * ck8_step(eb[i]);
-        out[row * cols + col] = GELU_BWD ? dy[row * cols + col] * act_grad(ACT_GELU, v) : v;
+__device__ __forceinline__ float read_value(float v, float dy) { return GELU_BWD ? dy * act_grad(ACT_GELU, v) : v; }
+
+template <bool GELU_BWD>
+__global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __restrict__ q, const unsigned char* __restrict__ eb, const float4* __restrict__ dy,
+                                                            float4* __restrict__ out, int64_t quads) {
+    const int64_t first = (int64_t)blockIdx.x * (kThreads * kAhead) + threadIdx.x;
+    unsigned w[kAhead], byte[kAhead];
+    float4 d[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        const int64_t at = first + i * kThreads;
+        if (at >= quads) break;
+        w[i] = __ldcs(q + at), byte[i] = __ldg(eb + (at >> 3));
+        if (GELU_BWD) d[i] = __ldcs(dy + at);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        const int64_t at = first + i * kThreads;
+        if (at >= quads) break;
+        const float step = ck8_step(byte[i]);
+        float4 o;
+        o.x = read_value<GELU_BWD>((float)(signed char)w[i] * step, GELU_BWD ? d[i].x : 0.0f);
+        o.y = read_value<GELU_BWD>((float)(signed char)(w[i] >> 8) * step, GELU_BWD ? d[i].y : 0.0f);
+        o.z = read_value<GELU_BWD>((float)(signed char)(w[i] >> 16) * step, GELU_BWD ? d[i].z : 0.0f);
+        o.w = read_value<GELU_BWD>((float)(signed char)(w[i] >> 24) * step, GELU_BWD ? d[i].w : 0.0f);
+        __stcs(out + at, o);
     }
 }
 
-static int grid_for(int64_t rows, int64_t cols, int sm_count) {
-    const int64_t need = (rows * ck8_groups(cols) + kThreads / 32 - 1) / (kThreads / 32), most = 16 * (int64_t)sm_count;
-    return (int)(need < most ? need : most);
+// Any columns, any alignment: a warp per group, a lane per column, four groups of a warp in flight.
+__global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__ x, char* __restrict__ ck, int64_t rows, int64_t cols) {
+    const int lane = threadIdx.x & 31;
+    const int64_t groups = ck8_groups(cols), total = rows * groups;
+    const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAhead;
+    unsigned char* eb = reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols);
+    int64_t row = first / groups, g = first - row * groups, at[kAhead];
+    float v[kAhead];
+    bool ok[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        ok[i] = first + i < total && g * kGroup + lane < cols;
+        at[i] = row * cols + g * kGroup + lane;
+        v[i] = ok[i] ? __ldcs(x + at[i]) : 0.0f;
+        if (++g == groups) g = 0, row++;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        if (first + i >= total) break;
+        const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
+        if (ok[i]) ck[at[i]] = (char)ck8_quantise(v[i], byte);
+        if (lane == 0) eb[first + i] = (unsigned char)byte;
+    }
 }
 
-cudaError_t launch_ck8_save(const float* x, char* ck, int64_t rows, int64_t cols, int sm_count, cudaStream_t st) {
-    k_ck8_save<<<grid_for(rows, cols, sm_count), kThreads, 0, st>>>(x, ck, rows, cols);
+template <bool GELU_BWD>
+__global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ ck, const float* __restrict__ dy, float* __restrict__ out, int64_t rows,
+                                                       int64_t cols) {
+    const int lane = threadIdx.x & 31;
+    const int64_t groups = ck8_groups(cols), total = rows * groups;
+    const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAhead;
+    const unsigned char* eb = reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols);
+    int64_t row = first / groups, g = first - row * groups, at[kAhead];
+    float d[kAhead];
+    int q[kAhead];
+    unsigned byte[kAhead];
+    bool ok[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+        ok[i] = first + i < total && g * kGroup + lane < cols;
+        at[i] = row * cols + g * kGroup + lane;
+        q[i] = ok[i] ? (signed char)__ldcs(ck + at[i]) : 0;
+        byte[i] = ok[i] ? __ldg(eb + first + i) : 0u;
+        d[i] = GELU_BWD && ok[i] ? __ldcs(dy + at[i]) : 0.0f;
+        if (++g == groups) g = 0, row++;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+        if (ok[i]) __stcs(out + at[i], read_value<GELU_BWD>((float)q[i] * ck8_step(byte[i]), d[i]));
+}
+
+static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+static bool wide(int64_t cols, const void* ck, const float* a, const float* b) { return cols % kGroup == 0 && aligned(ck, 4) && aligned(a, 16) && aligned(b, 16); }
+static unsigned wide_grid(int64_t rows, int64_t cols) { return (unsigned)((rows * cols / 4 + kThreads * kAhead - 1) / (kThreads * kAhead)); }
+static unsigned any_grid(int64_t rows, int64_t cols) {
+    const int64_t per_block = kThreads / 32 * kAhead;
+    return (unsigned)((rows * ck8_groups(cols) + per_block - 1) / per_block);
+}
+
+cudaError_t launch_ck8_save(const float* x, char* ck, int64_t rows, int64_t cols, cudaStream_t st) {
+    if (wide(cols, ck, x, nullptr))
+        k_ck8_save_wide<<<wide_grid(rows, cols), kThreads, 0, st>>>(reinterpret_cast<const float4*>(x), reinterpret_cast<unsigned*>(ck),
+                                                                  reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols), rows * cols / 4);
+    else
+        k_ck8_save<<<any_grid(rows, cols), kThreads, 0, st>>>(x, ck, rows, cols);
     return cudaPeekAtLastError();
 }
-cudaError_t launch_ck8_load(const char* ck, float* x, int64_t rows, int64_t cols, int sm_count, cudaStream_t st) {
-    k_ck8_read<false><<<grid_for(rows, cols, sm_count), kThreads, 0, st>>>(ck, nullptr, x, rows, cols);
+template <bool GELU_BWD>
+static cudaError_t launch_read(const char* ck, const float* dy, float* out, int64_t rows, int64_t cols, cudaStream_t st) {
+    if (wide(cols, ck, dy, out))
+        k_ck8_read_wide<GELU_BWD><<<wide_grid(rows, cols), kThreads, 0, st>>>(reinterpret_cast<const unsigned*>(ck),
+                                                                            reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols),
+                                                                            reinterpret_cast<const float4*>(dy), reinterpret_cast<float4*>(out), rows * cols / 4);
+    else
+        k_ck8_read<GELU_BWD><<<any_grid(rows, cols), kThreads, 0, st>>>(ck, dy, out, rows, cols);
     return cudaPeekAtLastError();
 }
-cudaError_t launch_ck8_gelu_bwd(const char* ck, const float* dy, float* dx, int64_t rows, int64_t cols, int sm_count, cudaStream_t st) {
-    k_ck8_read<true><<<grid_for(rows, cols, sm_count), kThreads, 0, st>>>(ck, dy, dx, rows, cols);
-    return cudaPeekAtLastError();
+cudaError_t launch_ck8_load(const char* ck, float* x, int64_t rows, int64_t cols, cudaStream_t st) { return launch_read<false>(ck, nullptr, x, rows, cols, st); }
+cudaError_t launch_ck8_gelu_bwd(const char* ck, const float* dy, float* dx, int64_t rows, int64_t cols, cudaStream_t st) {
+    return launch_read<true>(ck, dy, dx, rows, cols, st);
 }
 
 }  // namespace slb_ffn

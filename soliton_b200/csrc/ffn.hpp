@@ -92,6 +92,7 @@ struct GemmArgs {
     float *save, *save2;            // pre-activations in fp32 ...
     char *save8, *save8_2;          // ... or as checkpoints
     int gate_blocks;                // EPI_GATED: blocks of the gate's weight; the second weight's follow in the plane
+    int64_t groups, exp_offset;     // set by launch_gemm: of the checkpoints
     int wide;                       // set by launch_gemm: rows and pointers allow 16-byte accesses (4-byte for checkpoints)
 };
 
@@ -110,48 +111,62 @@ inline __host__ __device__ int64_t ck8_exp_offset(int64_t rows, int64_t cols) { 
 inline __host__ __device__ int64_t ck8_bytes(int64_t rows, int64_t cols) {
     return ck8_exp_offset(rows, cols) + rows * ck8_groups(cols);
 }
-cudaError_t launch_ck8_save(const float* x, char* ck, int64_t rows, int64_t cols, int sm_count, cudaStream_t st);
-cudaError_t launch_ck8_load(const char* ck, float* x, int64_t rows, int64_t cols, int sm_count, cudaStream_t st);
-cudaError_t launch_ck8_gelu_bwd(const char* ck, const float* dy, float* dx, int64_t rows, int64_t cols, int sm_count, cudaStream_t st);
+cudaError_t launch_ck8_save(const float* x, char* ck, int64_t rows, int64_t cols, cudaStream_t st);
+cudaError_t launch_ck8_load(const char* ck, float* x, int64_t rows, int64_t cols, cudaStream_t st);
+cudaError_t launch_ck8_gelu_bwd(const char* ck, const float* dy, float* dx, int64_t rows, int64_t cols, cudaStream_t st);
 
 #ifdef __CUDACC__
 // The exponent byte of a group whose largest magnitude has these bits (sign cleared): the smallest e >= -126 with
 // 127 * 2^e >= the magnitude, plus 127; 255 when the group holds an infinity or a NaN. In a normal magnitude
 // 1.f * 2^p, 127 * 2^(p - 6) = 1.984375 * 2^p suffices up to f = 0.984375 and 2^(p - 5) is needed beyond.
 __device__ __forceinline__ unsigned ck8_exponent(unsigned bits) {
-    if (bits >= 0x7f800000u) return 255u;
-    const int p = (int)(bits >> 23) - 127;
-    const int e = p - 6 + ((bits & 0x7fffffu) > 0x7e0000u ? 1 : 0);
-    return (unsigned)((e < -126 ? -126 : e) + 127);
+    const unsigned byte = max((bits + 0x1ffffu) >> 23, 7u) - 6u;  // the addition carries into the exponent for f beyond 0.984375
+    return bits >= 0x7f800000u ? 255u : byte;
 }
 // 2^(byte - 127) for bytes 1..254; a byte of 0 stands for 2^-127; 255 gives NaN.
 __device__ __forceinline__ float ck8_step(unsigned byte) {
     return byte == 255u ? __int_as_float(0x7fc00000) : byte == 0u ? __int_as_float(0x00400000) : __int_as_float((int)(byte << 23));
 }
 // The reciprocal step, a power of two as well: bytes that ck8_exponent gives are 1..249, so 254 - byte is 5..253.
-__device__ __forceinline__ float ck8_inv_step(unsigned byte) { return byte == 255u ? 0.0f : __int_as_float((int)((254u - byte) << 23)); }
-// Nearest multiple of the step, ties to even; |x| <= 127 steps by the choice of the exponent. Groups marked 255 store 0.
-__device__ __forceinline__ int ck8_quantise(float x, float inv_step, unsigned byte) { return byte == 255u ? 0 : __float2int_rn(x * inv_step); }
+__device__ __forceinline__ float ck8_inv_step(unsigned byte) { return __int_as_float((int)(((254u - byte) & 255u) << 23)); }
+// Nearest multiple of the step, ties to even, in the low byte; |x| <= 127 steps by the choice of the exponent. x * inv_step
+// is exact, and the sum with 1.5 * 2^23 has the integer, rounded, in its low bits. Groups marked 255 store zeros.
+__device__ __forceinline__ unsigned ck8_quantise(float x, unsigned byte) {
+    return byte == 255u ? 0u : (unsigned)__float_as_int(fmaf(x, ck8_inv_step(byte), 12582912.0f));
+}
+__device__ __forceinline__ unsigned ck8_quantise4(float x, float y, float z, float w, unsigned byte) {
+    const float inv = ck8_inv_step(byte);
+    const unsigned lo = __byte_perm(__float_as_uint(fmaf(x, inv, 12582912.0f)), __float_as_uint(fmaf(y, inv, 12582912.0f)), 0x0040);
+    const unsigned hi = __byte_perm(__float_as_uint(fmaf(z, inv, 12582912.0f)), __float_as_uint(fmaf(w, inv, 12582912.0f)), 0x0040);
+    return byte == 255u ? 0u : __byte_perm(lo, hi, 0x5410);
+}
 
-// Two ulps at most each, as CUDA documents them; what an argument's rounding adds is relative to terms that vanish with it.
-__device__ __forceinline__ float fast_exp(float v) { return __expf(v); }
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + fast_exp(-v)); }
-
+// exp and quotients to about two ulps; what an argument's rounding adds is relative to terms that vanish with it.
+__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+// Phi(v) and e = exp(-v^2 / 2). 1 - erf(z) = (a1 t + ... + a5 t^5) exp(-z^2) with t = 1 / (1 + p z), for z >= 0 (Abramowitz and
+// Stegun 7.1.26), is off by 1.5e-7 at most, which Phi halves: about an ulp of a value near one, at under half the
+// instructions of erff, whose cost showed (30 k cycles a tile of 128 x 256 against 24 k), and the derivative needs e anyway.
+__device__ __forceinline__ float normal_cdf(float v, float& e) {
+    const float z = fabsf(v) * 0.70710678f;
+    e = __expf(-0.5f * v * v);
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * e;  // Phi(-|v|)
+    return v < 0.0f ? tail : 1.0f - tail;
+}
 __device__ __forceinline__ float act_of(int act, float v) {
-    if (act == ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    if (act == ACT_GELU) {
+        float e;
+        return v * normal_cdf(v, e);
+    }
     if (act == ACT_SILU) return v * sigmoid(v);
     return v;
 }
-// GELU' = Phi(v) + v phi(v). Both share exp(-v^2 / 2): 1 - erf(z) = (a1 t + ... + a5 t^5) exp(-z^2), t = 1 / (1 + p z), for z >= 0
-// (Abramowitz and Stegun 7.1.26), off by 1.5e-7 at most, which Phi halves: about an ulp of a derivative near one, at under
-// half the instructions of erff and expf apart.
 __device__ __forceinline__ float act_grad(int act, float v) {
-    if (act == ACT_GELU) {
-        const float z = fabsf(v) * 0.70710678f, e = fast_exp(-0.5f * v * v);
-        const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
-        const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        const float tail = 0.5f * poly * e;                     // Phi(-|v|)
-        return fmaf(v * 0.39894228f, e, v < 0.0f ? tail : 1.0f - tail);
+    if (act == ACT_GELU) {  // Phi(v) + v phi(v)
+        float e;
+        const float cdf = normal_cdf(v, e);
+        return fmaf(v * 0.39894228f, e, cdf);
     }
     if (act == ACT_SILU) {
         const float sig = sigmoid(v);

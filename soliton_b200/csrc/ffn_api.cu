@@ -432,7 +432,7 @@ int slb_ck8_save(int dev, const float* x, void* ck, int64_t rows, int64_t cols) 
     Op op;
     if (!op.ok) return -1;
     op.reads(x, 4 * rows * cols), op.writes(ck, ck8_bytes(rows, cols));
-    op.launched(launch_ck8_save(x, static_cast<char*>(ck), rows, cols, op.sms(), 0));
+    op.launched(launch_ck8_save(x, static_cast<char*>(ck), rows, cols, 0));
     return op.done();
 }
 int slb_ck8_load(int dev, const void* ck, float* x, int64_t rows, int64_t cols) {
@@ -441,7 +441,7 @@ int slb_ck8_load(int dev, const void* ck, float* x, int64_t rows, int64_t cols) 
     Op op;
     if (!op.ok) return -1;
     op.reads(ck, ck8_bytes(rows, cols)), op.writes(x, 4 * rows * cols);
-    op.launched(launch_ck8_load(static_cast<const char*>(ck), x, rows, cols, op.sms(), 0));
+    op.launched(launch_ck8_load(static_cast<const char*>(ck), x, rows, cols, 0));
     return op.done();
 }
 int slb_ck8_gelu_bwd(int dev, const void* ck, const float* dy, float* dx, int64_t rows, int64_t cols) {
@@ -450,7 +450,7 @@ int slb_ck8_gelu_bwd(int dev, const void* ck, const float* dy, float* dx, int64_
     Op op;
     if (!op.ok) return -1;
     op.reads(ck, ck8_bytes(rows, cols)), op.reads(dy, 4 * rows * cols), op.writes(dx, 4 * rows * cols);
-    op.launched(launch_ck8_gelu_bwd(static_cast<const char*>(ck), dy, dx, rows, cols, op.sms(), 0));
+    op.launched(launch_ck8_gelu_bwd(static_cast<const char*>(ck), dy, dx, rows, cols, 0));
     return op.done();
 }
 

@@ -191,134 +191,110 @@ __device__ __forceinline__ int turned(int row, int chunk) {
     return (row * kChunksPerRow + (chunk ^ (row & 7))) * 4;
 }
 
-// Where pre-activations go: the addresses of this lane's next element, in fp32 and as a checkpoint (null: not kept).
-struct Keep {
-    float* full;
-    char* q;            // a lane's bytes
-    char* exp;          // the row's exponent byte
-    __device__ __forceinline__ Keep(const GemmArgs& g, float* f, char* ck, int64_t row, int64_t col) {
-        full = f ? f + row * g.cols + col : nullptr;
-        q = ck ? ck + row * g.cols + col : nullptr;
-        exp = ck ? ck + ck8_exp_offset(g.rows, g.cols) + row * ck8_groups(g.cols) + col / kGroup : nullptr;
-    }
-    __device__ __forceinline__ void next(int64_t elements, int64_t groups) {
-        if (full) full += elements;
-        if (q) q += elements, exp += groups;
-    }
-    // four columns; eight neighbouring lanes hold the group
-    __device__ __forceinline__ void put4(const float4& v, int lane) const {
-        if (full) *reinterpret_cast<float4*>(full) = v;
-        if (q) {
-            unsigned top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
-                               max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+// Keeps pre-activations, in fp32, as a checkpoint, or both (null: not), at element `at` of the tensor and exponent byte
+// `group` of the checkpoint. Four columns: eight neighbouring lanes hold the group.
+__device__ __forceinline__ void keep4(const float4& v, int64_t at, int64_t group, const GemmArgs& g, float* full, char* ck, int lane) {
+    if (full) *reinterpret_cast<float4*>(full + at) = v;
+    if (ck) {
+        unsigned top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+                           max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffu << (lane & 24), top, o));
-            const unsigned byte = ck8_exponent(top);
-            const float inv = ck8_inv_step(byte);
-            *reinterpret_cast<unsigned*>(q) = (unsigned)(ck8_quantise(v.x, inv, byte) & 255) | (unsigned)(ck8_quantise(v.y, inv, byte) & 255) << 8 |
-                                              (unsigned)(ck8_quantise(v.z, inv, byte) & 255) << 16 | (unsigned)(ck8_quantise(v.w, inv, byte) & 255) << 24;
-            if ((lane & 7) == 0) *exp = (char)byte;
-        }
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffu << (lane & 24), top, o));
+        const unsigned byte = ck8_exponent(top);
+        *reinterpret_cast<unsigned*>(ck + at) = ck8_quantise4(v.x, v.y, v.z, v.w, byte);
+        if ((lane & 7) == 0) ck[g.exp_offset + group] = (char)byte;
     }
-    // one column; the warp holds the group
-    __device__ __forceinline__ void put1(float v, bool ok, int lane) const {
-        if (full && ok) *full = v;
-        if (q) {
-            const float x = ok ? v : 0.0f;
-            const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(x) & 0x7fffffffu));
-            if (ok) *q = (char)ck8_quantise(x, ck8_inv_step(byte), byte);
-            if (lane == 0) *exp = (char)byte;
-        }
+}
+// One column: the warp holds the group.
+__device__ __forceinline__ void keep1(float v, bool ok, int64_t at, int64_t group, const GemmArgs& g, float* full, char* ck, int lane) {
+    if (full && ok) full[at] = v;
+    if (ck) {
+        const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, ok ? __float_as_uint(v) & 0x7fffffffu : 0u));
+        if (ok) ck[at] = (char)ck8_quantise(v, byte);
+        if (lane == 0) ck[g.exp_offset + group] = (char)byte;
     }
-};
+}
 __device__ __forceinline__ float4 scaled(const float* p, float s1, float s2, const float4& bias) {
     const float4 v = *reinterpret_cast<const float4*>(p);
     return make_float4(fmaf(v.x * s1, s2, bias.x), fmaf(v.y * s1, s2, bias.y), fmaf(v.z * s1, s2, bias.z), fmaf(v.w * s1, s2, bias.w));
 }
 
 // The rows of a piece out of the turning buffer. Loops of a few rows, not straight code: the epilogue runs once per tile,
-// and code of its unrolled length spends its time fetching instructions (150 k cycles a tile); the activation is chosen
-// outside them and addresses advance, for what is left is bound by instructions issued.
+// and code of its unrolled length spends its time fetching instructions (150 k cycles a tile). The activation is chosen
+// outside them and one offset serves all tensors: what is left is bound by instructions issued, and 128 sums leave few
+// registers.
 template <int EPI, int ROWS, int ACT>
 __device__ __forceinline__ void finish_rows(const GemmArgs& g, const float* buf, const Piece& p, float s1, float s2, int lane) {
     const bool second = EPI == EPI_STORE && p.row0 >= g.split;
-    const int64_t first = p.row0 - (second ? g.split : 0), groups = ck8_groups(g.cols);
+    const int64_t first = p.row0 - (second ? g.split : 0);
+    float* out = second ? g.out2 : g.out;
+    constexpr int kAtOnce = EPI == EPI_LINEAR ? 2 : 4;
     if (g.wide && p.col0 + 32 <= g.cols) {  // 16-byte accesses: eight lanes a row, four rows at a time
         const int chunk = lane & 7;
-        const int64_t col = p.col0 + chunk * 4, row = first + (lane >> 3), step = 4 * g.cols;
+        const int64_t col = p.col0 + chunk * 4, row = first + (lane >> 3);
         const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         const float4 bias = EPI != EPI_STORE && g.bias ? __ldg(reinterpret_cast<const float4*>(g.bias + col)) : none;
         const float4 bias2 = EPI == EPI_GATED && g.bias2 ? __ldg(reinterpret_cast<const float4*>(g.bias2 + col)) : none;
-        float* out = (second ? g.out2 : g.out) + row * g.cols + col;
-        const float* res = EPI == EPI_LINEAR && g.residual ? g.residual + row * g.cols + col : nullptr;
-        Keep keep(g, EPI == EPI_STORE ? nullptr : g.save, EPI == EPI_STORE ? nullptr : g.save8, row, col);
-        Keep keep2(g, EPI == EPI_GATED ? g.save2 : nullptr, EPI == EPI_GATED ? g.save8_2 : nullptr, row, col);
+        int64_t at = row * g.cols + col, group = EPI == EPI_STORE ? 0 : row * g.groups + col / kGroup;
 #pragma unroll 1
-        for (int r0 = lane >> 3; r0 < ROWS; r0 += 16) {
-            float4 add[4];
-            if (EPI == EPI_LINEAR && res) {
+        for (int r0 = lane >> 3; r0 < ROWS; r0 += 4 * kAtOnce) {
+            float4 add[kAtOnce];
+            if (EPI == EPI_LINEAR && g.residual) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) add[i] = r0 + 4 * i < p.rows ? *reinterpret_cast<const float4*>(res + i * step) : none;
-                res += 4 * step;
+                for (int i = 0; i < kAtOnce; i++) add[i] = r0 + 4 * i < p.rows ? *reinterpret_cast<const float4*>(g.residual + at + 4 * i * g.cols) : none;
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < kAtOnce; i++) {
                 const int r = r0 + 4 * i;
-                float4 v = scaled(buf + turned<EPI>(r, chunk), s1, s2, bias), w = none;
-                if (EPI == EPI_GATED) w = scaled(buf + turned<EPI>(r, 8 + chunk), s1, s2, bias2);
-                const bool there = r < p.rows;  // the same for the eight lanes of a row
-                if (EPI != EPI_STORE) {
-                    if (there) keep.put4(v, lane);
-                    keep.next(step, 4 * groups);
-                    v = make_float4(act_of(ACT, v.x), act_of(ACT, v.y), act_of(ACT, v.z), act_of(ACT, v.w));
+                if (r < p.rows) {  // the same for the eight lanes of a row
+                    float4 v = scaled(buf + turned<EPI>(r, chunk), s1, s2, bias);
+                    if (EPI != EPI_STORE) {
+                        keep4(v, at, group, g, g.save, g.save8, lane);
+                        v = make_float4(act_of(ACT, v.x), act_of(ACT, v.y), act_of(ACT, v.z), act_of(ACT, v.w));
+                    }
+                    if (EPI == EPI_GATED) {
+                        const float4 w = scaled(buf + turned<EPI>(r, 8 + chunk), s1, s2, bias2);
+                        keep4(w, at, group, g, g.save2, g.save8_2, lane);
+                        v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
+                    }
+                    if (EPI == EPI_LINEAR && g.residual) v = make_float4(v.x + add[i].x, v.y + add[i].y, v.z + add[i].z, v.w + add[i].w);
+                    *reinterpret_cast<float4*>(out + at) = v;
                 }
-                if (EPI == EPI_GATED) {
-                    if (there) keep2.put4(w, lane);
-                    keep2.next(step, 4 * groups);
-                    v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
-                }
-                if (EPI == EPI_LINEAR && res) v = make_float4(v.x + add[i].x, v.y + add[i].y, v.z + add[i].z, v.w + add[i].w);
-                if (there) *reinterpret_cast<float4*>(out) = v;
-                out += step;
+                at += 4 * g.cols, group += 4 * g.groups;
             }
         }
         return;
     }
-    const int64_t col = p.col0 + lane, step = g.cols;  // any alignment: a column per lane, eight rows' loads in flight
+    const int64_t col = p.col0 + lane;  // any alignment: a column per lane, several rows' loads in flight
     const bool ok = col < g.cols;
     const float bias = EPI != EPI_STORE && g.bias && ok ? __ldg(g.bias + col) : 0.0f;
     const float bias2 = EPI == EPI_GATED && g.bias2 && ok ? __ldg(g.bias2 + col) : 0.0f;
-    float* out = (second ? g.out2 : g.out) + first * g.cols + col;
-    const float* res = EPI == EPI_LINEAR && g.residual ? g.residual + first * g.cols + col : nullptr;
-    Keep keep(g, EPI == EPI_STORE ? nullptr : g.save, EPI == EPI_STORE ? nullptr : g.save8, first, col);
-    Keep keep2(g, EPI == EPI_GATED ? g.save2 : nullptr, EPI == EPI_GATED ? g.save8_2 : nullptr, first, col);
+    int64_t at = first * g.cols + col, group = EPI == EPI_STORE ? 0 : first * g.groups + p.col0 / kGroup;
 #pragma unroll 1
-    for (int r0 = 0; r0 < ROWS && r0 < p.rows; r0 += 8) {
-        float add[8];
-        if (EPI == EPI_LINEAR && res) {
+    for (int r0 = 0; r0 < ROWS && r0 < p.rows; r0 += 2 * kAtOnce) {
+        float add[2 * kAtOnce];
+        if (EPI == EPI_LINEAR && g.residual) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) add[i] = ok && r0 + i < p.rows ? res[i * step] : 0.0f;
-            res += 8 * step;
+            for (int i = 0; i < 2 * kAtOnce; i++) add[i] = ok && r0 + i < p.rows ? g.residual[at + i * g.cols] : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 2 * kAtOnce; i++) {
             const int r = r0 + i;
-            const bool there = r < p.rows;
-            float v = fmaf(buf[turned<EPI>(r, lane >> 2) + (lane & 3)] * s1, s2, bias), w = 0.0f;
-            if (EPI == EPI_GATED) w = fmaf(buf[turned<EPI>(r, 8 + (lane >> 2)) + (lane & 3)] * s1, s2, bias2);
-            if (EPI != EPI_STORE) {
-                if (there) keep.put1(v, ok, lane);
-                keep.next(step, groups);
-                v = act_of(ACT, v);
+            if (r < p.rows) {
+                float v = fmaf(buf[turned<EPI>(r, lane >> 2) + (lane & 3)] * s1, s2, bias);
+                if (EPI != EPI_STORE) {
+                    keep1(v, ok, at, group, g, g.save, g.save8, lane);
+                    v = act_of(ACT, v);
+                }
+                if (EPI == EPI_GATED) {
+                    const float w = fmaf(buf[turned<EPI>(r, 8 + (lane >> 2)) + (lane & 3)] * s1, s2, bias2);
+                    keep1(w, ok, at, group, g, g.save2, g.save8_2, lane);
+                    v *= w;
+                }
+                if (EPI == EPI_LINEAR && g.residual) v += add[i];
+                if (ok) out[at] = v;
             }
-            if (EPI == EPI_GATED) {
-                if (there) keep2.put1(w, ok, lane);
-                keep2.next(step, groups);
-                v *= w;
-            }
-            if (EPI == EPI_LINEAR && res) v += add[i];
-            if (there && ok) *out = v;
-            out += step;
+            at += g.cols, group += g.groups;
         }
     }
 }
@@ -617,6 +593,7 @@ cudaError_t launch_gemm(const GemmArgs& args, bool a_mn, bool b_mn, int pieces_b
     GemmArgs g = args;
     g.wide = g.cols % 4 == 0 && aligned(g.out, 16) && aligned(g.out2, 16) && aligned(g.bias, 16) && aligned(g.bias2, 16) && aligned(g.residual, 16) &&
              aligned(g.save, 16) && aligned(g.save2, 16) && aligned(g.save8, 4) && aligned(g.save8_2, 4);
+    g.groups = ck8_groups(g.cols), g.exp_offset = ck8_exp_offset(g.rows, g.cols);
     if (epi == EPI_LINEAR) return launch_sized<2, false, false, EPI_LINEAR>(g, sm_count, st);
     if (epi == EPI_GATED) return launch_sized<2, false, false, EPI_GATED>(g, sm_count, st);
     if (!a_mn && b_mn) return launch_sized<2, false, true, EPI_STORE>(g, sm_count, st);
