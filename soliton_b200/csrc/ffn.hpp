@@ -93,7 +93,7 @@ struct GemmArgs {
     char *save8, *save8_2;          // ... or as checkpoints
     int gate_blocks;                // EPI_GATED: blocks of the gate's weight; the second weight's follow in the plane
     int64_t groups, exp_offset;     // set by launch_gemm: of the checkpoints
-    int wide;                       // set by launch_gemm: rows and pointers allow 16-byte accesses (4-byte for checkpoints)
+    int wide;                       // set by launch_gemm: rows and pointers allow 16-byte accesses (8-byte for checkpoints)
 };
 
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
@@ -150,8 +150,8 @@ __device__ __forceinline__ float normal_cdf(float v, float& e) {
     const float z = fabsf(v) * 0.70710678f;
     e = __expf(-0.5f * v * v);
     const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * poly * e;  // Phi(-|v|)
+    // half the coefficients: tail = Phi(-|v|)
+    const float tail = e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
     return v < 0.0f ? tail : 1.0f - tail;
 }
 __device__ __forceinline__ float act_of(int act, float v) {

@@ -7,13 +7,12 @@
 // descriptors.
 //
 // The tensor cores round every accumulation towards zero, so a long sum drifts by about half an ulp per step. Sums are
-// therefore cut into segments of 256 along K: the accumulator has two buffers, the warps of the epilogue add a finished
+// therefore cut into segments of 256 to 384 along K: the accumulator has two buffers, the warps of the epilogue add a finished
 // segment to fp32 registers (to nearest) while the next one runs in the other buffer. The same double buffer lets a
 // tile's epilogue run under the next tile's products: blocks are persistent, one per SM.
 //
-// The epilogue transposes 32 x 32 pieces through shared memory so that a lane holds a column: bias, residual, saved
-// pre-activations and the result then move as full 128-byte lines at any alignment, and the 32 lanes of a row are one
-// group of a checkpoint.
+// The epilogue works on the accumulator's own arrangement, a row per lane and 32 columns at a time (one group of a
+// checkpoint), and turns pieces of 32 x 32 through shared memory to store them in whole lines.
 //
 // Every wait is bounded: a block whose wait runs out records ST_TIMEOUT_PRODUCT, waits (bounded) for its copies and
 // products in flight, frees its tensor memory and returns.
@@ -25,13 +24,13 @@ namespace slb_ffn {
 constexpr int BM = 128;
 constexpr int kEpiWarps = 8;
 constexpr int kGemmThreads = 128 + 32 * kEpiWarps;          // a warpgroup that copies and issues, two of the epilogue
-// Registers: three warpgroups start with 168 a thread, 504 in all; the first keeps 56 and the other two, which hold
-// 128 sums a thread, take 224 each: 504 again.
-constexpr int kIssueRegs = 56, kEpiRegs = 224;
+// Registers: three warpgroups start with 168 a thread, 504 in all; the first keeps 40 and the other two, which hold 128
+// sums a thread, take 232 each: 504 again. (Four warpgroups of 64 sums each were no faster and left no room for the epilogue.)
+constexpr int kIssueRegs = 40, kEpiRegs = 232;
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kTurnFloats = 32 * 32;                        // one warp's turning buffer
 constexpr int kSmemBytes = kRingBytes + kEpiWarps * kTurnFloats * 4 + 256 + 1024;
-constexpr int kSegment = 4;                                 // k-blocks per accumulator segment
+constexpr int kSegment = 4, kFirstSegments = 6;             // k-blocks per accumulator segment; in a tile's first two
 constexpr int kMaxStages = 4;
 constexpr int kGroupM = 8;                                  // row tiles that blocks walk side by side (reuse in L2)
 
@@ -134,18 +133,16 @@ __device__ __forceinline__ void give_up(const GemmArgs& g, volatile int* stop) {
     *stop = 1;
     if (g.status) *reinterpret_cast<volatile int*>(g.status) = slb::ST_TIMEOUT_PRODUCT;
 }
-__device__ __forceinline__ void tmem_load32(unsigned addr, float (&v)[32]) {
-    unsigned r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
-        "%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr));
+// Adds 16 columns of the warp's 32 rows of tensor memory to `sum`.
+__device__ __forceinline__ void tmem_add16(unsigned addr, float* sum) {
+    unsigned r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 16; i++) sum[i] += __uint_as_float(r[i]);
 }
 
 // Shared-memory descriptors of block images (128-byte swizzle, groups of eight 128-byte rows 1 KiB apart). K-major: a
@@ -166,13 +163,13 @@ __device__ __forceinline__ int blocks_wide(const GemmArgs& g, int n) {
     const int left = EPI == EPI_GATED ? 2 * (g.gate_blocks - n * (most / 2)) : g.b.mn_blocks - n * most;
     return left >= most ? most : (left + 1) & ~1;
 }
-// Where chunk c (32 columns) of a warp's half lies in a tile's accumulator. Gated: the first half of the chunks are columns
-// of the gate, the others the same columns of the second product, which follow 64 later.
+// Where chunk c (32 columns) of a warp's half lies in a tile's accumulator. Gated: by turns columns of the gate and the
+// same columns of the second product, which lie 64 further.
 template <int EPI, int CHUNKS>
 __device__ __forceinline__ constexpr unsigned column_of(int half, int c) {
     if (EPI != EPI_GATED) return (unsigned)(half * CHUNKS + c) * 32;
-    const int j = half * (CHUNKS / 2) + c % (CHUNKS / 2);
-    return (unsigned)((j >> 1) * 128 + (j & 1) * 32 + (c >= CHUNKS / 2 ? 64 : 0));
+    const int j = half * (CHUNKS / 2) + c / 2;
+    return (unsigned)((j >> 1) * 128 + (j & 1) * 32 + (c & 1) * 64);
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -182,130 +179,171 @@ struct Piece {          // rows x 32 columns of the output
     int rows;           // that exist
 };
 
-// A warp's 4 KiB turning buffer: 32 rows of 32 columns, or 16 of 64 for the gated pair, in 16-byte chunks whose place
-// within a row is exclusive-ored with the row's low bits, so that rows written by their lanes and rows read by eight lanes
-// both spread over all banks.
-template <int EPI>
-__device__ __forceinline__ int turned(int row, int chunk) {
-    constexpr int kChunksPerRow = EPI == EPI_GATED ? 16 : 8;
-    return (row * kChunksPerRow + (chunk ^ (row & 7))) * 4;
-}
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Keeps pre-activations, in fp32, as a checkpoint, or both (null: not), at element `at` of the tensor and exponent byte
-// `group` of the checkpoint. Four columns: eight neighbouring lanes hold the group.
-__device__ __forceinline__ void keep4(const float4& v, int64_t at, int64_t group, const GemmArgs& g, float* full, char* ck, int lane) {
-    if (full) *reinterpret_cast<float4*>(full + at) = v;
-    if (ck) {
-        unsigned top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
-                           max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+// The accumulator comes a row per lane, and that is how values are scaled, activated and put into checkpoints (32 columns
+// of a row are one group). To be stored they are turned: the warp's buffer is 4 KiB, 32 rows of 32 in 16-byte chunks
+// whose place within a row is exclusive-ored with the row's low bits, so that neither writing rows nor reading them
+// meets bank conflicts. Stored row per lane, a tensor took 8 k cycles a tile for its 32 lines an instruction. Under the
+// products, which read shared memory all the time, a load from it takes some 360 cycles: all of a piece are issued at once.
+__device__ __forceinline__ int turned(int row, int chunk) { return (row * 8 + (chunk ^ (row & 7))) * 4; }
+__device__ __forceinline__ void put_rows(const float (&v)[32], float* buf, int lane) {
+    __syncwarp();
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffu << (lane & 24), top, o));
+    for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(buf + turned(lane, i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+}
+// Stores a piece, plus `add` where given: eight lanes a row, four rows an instruction. at: the element of row 0, column 0.
+__device__ __forceinline__ void store_wide(const float (&v)[32], float* out, const float* add, int64_t at, int64_t cols, int rows, float* buf, int lane) {
+    const int64_t mine = at + (lane >> 3) * cols + (lane & 7) * 4;
+    const int left = rows - (lane >> 3);
+    float4 x[8];
+    if (add) {
+        float4 r[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = 4 * i < left ? *reinterpret_cast<const float4*>(add + mine + 4 * i * cols) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        put_rows(v, buf, lane);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = *reinterpret_cast<const float4*>(buf + turned(4 * i + (lane >> 3), lane & 7));
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = make_float4(x[i].x + r[i].x, x[i].y + r[i].y, x[i].z + r[i].z, x[i].w + r[i].w);
+    } else {
+        put_rows(v, buf, lane);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = *reinterpret_cast<const float4*>(buf + turned(4 * i + (lane >> 3), lane & 7));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (4 * i < left) *reinterpret_cast<float4*>(out + mine + 4 * i * cols) = x[i];
+}
+__device__ __forceinline__ void keep_wide(const float (&v)[32], const Piece& p, int64_t at, const GemmArgs& g, float* full, char* ck, float* buf, int lane) {
+    if (full) store_wide(v, full, nullptr, at, g.cols, p.rows, buf, lane);
+    if (ck && lane < p.rows) {
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) top = max(top, magnitude(v[i]));
         const unsigned byte = ck8_exponent(top);
-        *reinterpret_cast<unsigned*>(ck + at) = ck8_quantise4(v.x, v.y, v.z, v.w, byte);
-        if ((lane & 7) == 0) ck[g.exp_offset + group] = (char)byte;
+        char* q = ck + at + lane * g.cols;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint2*>(q + i) =
+                make_uint2(ck8_quantise4(v[i], v[i + 1], v[i + 2], v[i + 3], byte), ck8_quantise4(v[i + 4], v[i + 5], v[i + 6], v[i + 7], byte));
+        ck[g.exp_offset + (p.row0 + lane) * g.groups + p.col0 / kGroup] = (char)byte;
     }
 }
-// One column: the warp holds the group.
-__device__ __forceinline__ void keep1(float v, bool ok, int64_t at, int64_t group, const GemmArgs& g, float* full, char* ck, int lane) {
-    if (full && ok) full[at] = v;
-    if (ck) {
-        const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, ok ? __float_as_uint(v) & 0x7fffffffu : 0u));
-        if (ok) ck[at] = (char)ck8_quantise(v, byte);
-        if (lane == 0) ck[g.exp_offset + group] = (char)byte;
+__device__ __forceinline__ void scale_row(float (&v)[32], float s1, float s2, const float* bias) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+        const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[i] = fmaf(v[i] * s1, s2, b.x), v[i + 1] = fmaf(v[i + 1] * s1, s2, b.y);
+        v[i + 2] = fmaf(v[i + 2] * s1, s2, b.z), v[i + 3] = fmaf(v[i + 3] * s1, s2, b.w);
     }
 }
-__device__ __forceinline__ float4 scaled(const float* p, float s1, float s2, const float4& bias) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    return make_float4(fmaf(v.x * s1, s2, bias.x), fmaf(v.y * s1, s2, bias.y), fmaf(v.z * s1, s2, bias.z), fmaf(v.w * s1, s2, bias.w));
+template <int ACT>
+__device__ __forceinline__ void act_row(float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[i + j] = act_of(ACT, v[i + j]);
+        // eight at a time: all 32 side by side would not fit the registers
+        asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
+        if (i < 24)
+            asm volatile("" : "+f"(v[i + 8]), "+f"(v[i + 9]), "+f"(v[i + 10]), "+f"(v[i + 11]), "+f"(v[i + 12]), "+f"(v[i + 13]), "+f"(v[i + 14]), "+f"(v[i + 15]));
+    }
+}
+__device__ __forceinline__ void act_row(int act, float (&v)[32]) {
+    if (act == ACT_GELU) act_row<ACT_GELU>(v);
+    else if (act == ACT_SILU) act_row<ACT_SILU>(v);
+}
+// v: columns p.col0 to p.col0 + 31 of row p.row0 + lane (all 32 exist), w: the same of the gated block's second product.
+template <int EPI>
+__device__ __forceinline__ void finish_wide(const GemmArgs& g, float (&v)[32], float (&w)[32], const Piece& p, float s1, float s2, float* buf, int lane) {
+    const bool second = EPI == EPI_STORE && p.row0 >= g.split;
+    const int64_t at = (p.row0 - (second ? g.split : 0)) * g.cols + p.col0;
+    scale_row(v, s1, s2, EPI != EPI_STORE && g.bias ? g.bias + p.col0 : nullptr);
+    if (EPI != EPI_STORE) {
+        keep_wide(v, p, at, g, g.save, g.save8, buf, lane);
+        act_row(g.act, v);
+        if (EPI == EPI_GATED) {
+            scale_row(w, s1, s2, g.bias2 ? g.bias2 + p.col0 : nullptr);
+            keep_wide(w, p, at, g, g.save2, g.save8_2, buf, lane);
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[i] *= w[i];
+        }
+    }
+    store_wide(v, second ? g.out2 : g.out, EPI == EPI_LINEAR ? g.residual : nullptr, at, g.cols, p.rows, buf, lane);
 }
 
-// The rows of a piece out of the turning buffer. Loops of a few rows, not straight code: the epilogue runs once per tile,
-// and code of its unrolled length spends its time fetching instructions (150 k cycles a tile). The activation is chosen
-// outside them and one offset serves all tensors: what is left is bound by instructions issued, and 128 sums leave few
-// registers.
-template <int EPI, int ROWS, int ACT>
-__device__ __forceinline__ void finish_rows(const GemmArgs& g, const float* buf, const Piece& p, float s1, float s2, int lane) {
-    const bool second = EPI == EPI_STORE && p.row0 >= g.split;
-    const int64_t first = p.row0 - (second ? g.split : 0);
-    float* out = second ? g.out2 : g.out;
-    constexpr int kAtOnce = EPI == EPI_LINEAR ? 2 : 4;
-    if (g.wide && p.col0 + 32 <= g.cols) {  // 16-byte accesses: eight lanes a row, four rows at a time
-        const int chunk = lane & 7;
-        const int64_t col = p.col0 + chunk * 4, row = first + (lane >> 3);
-        const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float4 bias = EPI != EPI_STORE && g.bias ? __ldg(reinterpret_cast<const float4*>(g.bias + col)) : none;
-        const float4 bias2 = EPI == EPI_GATED && g.bias2 ? __ldg(reinterpret_cast<const float4*>(g.bias2 + col)) : none;
-        int64_t at = row * g.cols + col, group = EPI == EPI_STORE ? 0 : row * g.groups + col / kGroup;
-#pragma unroll 1
-        for (int r0 = lane >> 3; r0 < ROWS; r0 += 4 * kAtOnce) {
-            float4 add[kAtOnce];
-            if (EPI == EPI_LINEAR && g.residual) {
+// Any width, any alignment: turned so that a lane holds a column and a row leaves as one run of up to 128 bytes.
+__device__ __forceinline__ void turn(float (&v)[32], float* buf, int lane) {
+    put_rows(v, buf, lane);
 #pragma unroll
-                for (int i = 0; i < kAtOnce; i++) add[i] = r0 + 4 * i < p.rows ? *reinterpret_cast<const float4*>(g.residual + at + 4 * i * g.cols) : none;
-            }
+    for (int r = 0; r < 32; r++) v[r] = buf[turned(r, lane >> 2) + (lane & 3)];
+}
+// v[r]: this lane's column of row r
+__device__ __forceinline__ void keep_column(const float (&v)[32], int rows, bool ok, int64_t at, int64_t group, const GemmArgs& g, float* full, char* ck, int lane) {
+    if (full) {
 #pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {
-                const int r = r0 + 4 * i;
-                if (r < p.rows) {  // the same for the eight lanes of a row
-                    float4 v = scaled(buf + turned<EPI>(r, chunk), s1, s2, bias);
-                    if (EPI != EPI_STORE) {
-                        keep4(v, at, group, g, g.save, g.save8, lane);
-                        v = make_float4(act_of(ACT, v.x), act_of(ACT, v.y), act_of(ACT, v.z), act_of(ACT, v.w));
-                    }
-                    if (EPI == EPI_GATED) {
-                        const float4 w = scaled(buf + turned<EPI>(r, 8 + chunk), s1, s2, bias2);
-                        keep4(w, at, group, g, g.save2, g.save8_2, lane);
-                        v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
-                    }
-                    if (EPI == EPI_LINEAR && g.residual) v = make_float4(v.x + add[i].x, v.y + add[i].y, v.z + add[i].z, v.w + add[i].w);
-                    *reinterpret_cast<float4*>(out + at) = v;
-                }
-                at += 4 * g.cols, group += 4 * g.groups;
-            }
-        }
-        return;
+        for (int r = 0; r < 32; r++)
+            if (ok && r < rows) full[at + r * g.cols] = v[r];
     }
-    const int64_t col = p.col0 + lane;  // any alignment: a column per lane, several rows' loads in flight
-    const bool ok = col < g.cols;
-    const float bias = EPI != EPI_STORE && g.bias && ok ? __ldg(g.bias + col) : 0.0f;
-    const float bias2 = EPI == EPI_GATED && g.bias2 && ok ? __ldg(g.bias2 + col) : 0.0f;
-    int64_t at = first * g.cols + col, group = EPI == EPI_STORE ? 0 : first * g.groups + p.col0 / kGroup;
-#pragma unroll 1
-    for (int r0 = 0; r0 < ROWS && r0 < p.rows; r0 += 2 * kAtOnce) {
-        float add[2 * kAtOnce];
-        if (EPI == EPI_LINEAR && g.residual) {
+    if (ck) {
 #pragma unroll
-            for (int i = 0; i < 2 * kAtOnce; i++) add[i] = ok && r0 + i < p.rows ? g.residual[at + i * g.cols] : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * kAtOnce; i++) {
-            const int r = r0 + i;
-            if (r < p.rows) {
-                float v = fmaf(buf[turned<EPI>(r, lane >> 2) + (lane & 3)] * s1, s2, bias);
-                if (EPI != EPI_STORE) {
-                    keep1(v, ok, at, group, g, g.save, g.save8, lane);
-                    v = act_of(ACT, v);
-                }
-                if (EPI == EPI_GATED) {
-                    const float w = fmaf(buf[turned<EPI>(r, 8 + (lane >> 2)) + (lane & 3)] * s1, s2, bias2);
-                    keep1(w, ok, at, group, g, g.save2, g.save8_2, lane);
-                    v *= w;
-                }
-                if (EPI == EPI_LINEAR && g.residual) v += add[i];
-                if (ok) out[at] = v;
-            }
-            at += g.cols, group += g.groups;
+        for (int r = 0; r < 32; r++) {
+            if (r >= rows) continue;  // the same for the whole warp
+            const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, ok ? magnitude(v[r]) : 0u));
+            if (ok) ck[at + r * g.cols] = (char)ck8_quantise(v[r], byte);
+            if (lane == 0) ck[g.exp_offset + group + r * g.groups] = (char)byte;
         }
     }
 }
-template <int EPI, int ROWS>
-__device__ __forceinline__ void finish_piece(const GemmArgs& g, const float* buf, const Piece& p, float s1, float s2, int lane) {
-    if (EPI == EPI_STORE || g.act == ACT_NONE) finish_rows<EPI, ROWS, ACT_NONE>(g, buf, p, s1, s2, lane);
-    else if (g.act == ACT_GELU) finish_rows<EPI, ROWS, ACT_GELU>(g, buf, p, s1, s2, lane);
-    else finish_rows<EPI, ROWS, ACT_SILU>(g, buf, p, s1, s2, lane);
+template <int EPI>
+__device__ __forceinline__ void finish_any(const GemmArgs& g, float (&v)[32], float (&w)[32], const Piece& p, float s1, float s2, float* buf, int lane) {
+    const bool second = EPI == EPI_STORE && p.row0 >= g.split;
+    const int64_t row = p.row0 - (second ? g.split : 0), col = p.col0 + lane, at = row * g.cols + col;
+    const bool ok = col < g.cols;
+    float* out = (second ? g.out2 : g.out) + at;
+    turn(v, buf, lane);
+    const float bias = EPI != EPI_STORE && g.bias && ok ? __ldg(g.bias + col) : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 32; r++) v[r] = fmaf(v[r] * s1, s2, bias);
+    if (EPI != EPI_STORE) {
+        const int64_t group = row * g.groups + p.col0 / kGroup;
+        keep_column(v, p.rows, ok, at, group, g, g.save, g.save8, lane);
+        act_row(g.act, v);
+        if (EPI == EPI_GATED) {
+            turn(w, buf, lane);
+            const float bias2 = g.bias2 && ok ? __ldg(g.bias2 + col) : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 32; r++) w[r] = fmaf(w[r] * s1, s2, bias2);
+            keep_column(w, p.rows, ok, at, group, g, g.save2, g.save8_2, lane);
+#pragma unroll
+            for (int r = 0; r < 32; r++) v[r] *= w[r];
+        }
+        if (EPI == EPI_LINEAR && g.residual) {
+            const float* res = g.residual + at;
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += 16) {
+                float add[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) add[i] = ok && r0 + i < p.rows ? res[(r0 + i) * g.cols] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[r0 + i] += add[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 32; r++)
+        if (ok && r < p.rows) out[r * g.cols] = v[r];
 }
 
 // ---------------------------------------------------------------- the kernel
+
+// A segment's end. The first two of a tile are longer: the products can run that far ahead of the previous tile's epilogue.
+__device__ __forceinline__ int segment_end(int k0, int k_blocks) {
+    if (k_blocks <= 2 * kFirstSegments) return k0 == 0 ? (k_blocks + 1) / 2 : k_blocks;
+    return min(k0 + (k0 < 2 * kFirstSegments ? kFirstSegments : kSegment), k_blocks);
+}
 
 struct Tile {
     int m, n;
@@ -320,10 +358,10 @@ __device__ __forceinline__ Tile tile_at(int t, int m_tiles, int n_tiles) {
 // and 128 columns' worth of B in its shared memory and 128 rows of the accumulator, and the first issues products that
 // read both. Per value fetched a pair computes twice as much, which is what bounds large products: fetching from L2.
 // Warp 0 copies, warp 1 issues the products (in a pair's second block: reports arrived stages to the first), warps 4 to
-// 11 read the accumulators: two per 32 rows, each half the columns.
+// 11 read the accumulators: two per 32 rows, half the columns each.
 template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs g) {
-    constexpr int BN = 128 * CTAS, kBlocksN = BN / kBlock, kHalf = BN / 2, kChunks = kHalf / 32;
+    constexpr int BN = 128 * CTAS, kBlocksN = BN / kBlock, kChunks = BN / 64;  // chunks of 32 columns a warp
     constexpr int kOperandBytes = 2 * (int)kImageBytes;  // one piece of this block's 128 rows of A, or of its share of B
     constexpr int kStageBytes = (2 + PB) * kOperandBytes;
     constexpr int kStages = kRingBytes / kStageBytes < kMaxStages ? kRingBytes / kStageBytes : kMaxStages;
@@ -416,14 +454,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                 const Tile at = tile_at(t, g.m_tiles, g.n_tiles);
                 const unsigned idesc = 1u << 4 | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | (unsigned)(blocks_wide<CTAS, EPI>(g, at.n) * kBlock >> 3) << 17 |
                                        (unsigned)(BM * CTAS >> 4) << 24;
-                for (int k0 = 0; ok && k0 < g.k_blocks; k0 += kSegment, seg++) {
+                for (int k0 = 0, k1; ok && k0 < g.k_blocks; k0 = k1, seg++) {
+                    k1 = segment_end(k0, g.k_blocks);
                     const unsigned buf = seg & 1, d = tmem + buf * BN;
                     if (!mbar_wait<CTAS == 2>(tempty + 8 * buf, ((seg >> 1) & 1) ^ 1, g.timeout_ns, stop)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const int k1 = min(k0 + kSegment, g.k_blocks);
                     for (int kb = k0; kb < k1; kb++, it++) {
                         const unsigned s = it % kStages;
                         if (!mbar_wait(full + 8 * s, (it / kStages) & 1, g.timeout_ns, stop) ||
@@ -433,14 +471,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                         }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const unsigned at_a = ring_at + s * kStageBytes, at_b = at_a + 2 * kOperandBytes;
+                        const uint64_t a_hi = descriptor<AMN>(at_a), a_lo = descriptor<AMN>(at_a + kOperandBytes);
+                        const uint64_t b_hi = descriptor<BMN>(at_b), b_lo = descriptor<BMN>(at_b + kOperandBytes);
 #pragma unroll
-                        for (int product = 0; product < 1 + PB; product++) {  // hi*hi, lo*hi, hi*lo
-                            const uint64_t da = descriptor<AMN>(at_a + (product == 1 ? kOperandBytes : 0));
-                            const uint64_t db = descriptor<BMN>(at_b + (product == 2 ? kOperandBytes : 0));
-#pragma unroll
-                            for (int step = 0; step < kBlock / 16; step++)
-                                mma_f16<CTAS>(d, da + (uint64_t)(step * kStepBytes<AMN> >> 4), db + (uint64_t)(step * kStepBytes<BMN> >> 4), idesc,
-                                              !(kb == k0 && product == 0 && step == 0));
+                        for (int step = 0; step < kBlock / 16; step++) {
+                            const uint64_t da = (uint64_t)(step * kStepBytes<AMN> >> 4), db = (uint64_t)(step * kStepBytes<BMN> >> 4);
+                            mma_f16<CTAS>(d, a_lo + da, b_hi + db, idesc, !(kb == k0 && step == 0));
+                            mma_f16<CTAS>(d, a_hi + da, b_hi + db, idesc, 1);
+                            if (PB == 2) mma_f16<CTAS>(d, a_hi + da, b_lo + db, idesc, 1);
                         }
                         mma_commit<CTAS>(empty + 8 * s);
                     }
@@ -482,22 +520,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 32; i++) acc[c][i] = 0.0f;
             if (EPI == EPI_LINEAR && g.residual) {  // into L2 while the products run: a lane a row, this warp's columns
-                const int64_t row = (int64_t)(at.m * CTAS + rank) * BM + q * 32 + lane, col = (int64_t)at.n * BN + half * kHalf;
+                const int64_t row = (int64_t)(at.m * CTAS + rank) * BM + q * 32 + lane, col = (int64_t)at.n * BN + half * kChunks * 32;
                 if (row < g.rows)
-                    for (int64_t c = col; c < min(col + kHalf, g.cols); c += 32)
+                    for (int64_t c = col; c < min(col + kChunks * 32, g.cols); c += 32)
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(g.residual + row * g.cols + c));
             }
-            for (int k0 = 0; k0 < g.k_blocks; k0 += kSegment, seg++) {
+            for (int k0 = 0; k0 < g.k_blocks; k0 = segment_end(k0, g.k_blocks), seg++) {
                 const unsigned b = seg & 1;
                 ok = __all_sync(0xffffffffu, mbar_wait(tfull + 8 * b, (seg >> 1) & 1, g.timeout_ns, stop));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int c = 0; c < kChunks; c++) {
-                    float v[32];
-                    tmem_load32(tmem + ((unsigned)(q * 32) << 16) + b * BN + column_of<EPI, kChunks>(half, c), v);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) acc[c][i] += v[i];
+                    const unsigned from = tmem + ((unsigned)(q * 32) << 16) + b * BN + column_of<EPI, kChunks>(half, c);
+                    tmem_add16(from, acc[c]), tmem_add16(from + 16, acc[c] + 16);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
@@ -513,42 +549,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             if (EPI == EPI_STORE && p.row0 >= g.split) left += g.split;
             p.rows = left < 0 ? 0 : left < 32 ? (int)left : 32;
             if (p.rows == 0) continue;
-            const int all_rows = p.rows;
-            const int64_t row0 = p.row0;
+            // In place and in a loop that moves the next chunk up: registers are short, and so should the code be, which runs
+            // once per tile and is bound by fetching it when it is long (150 k cycles a tile for four chunks in a row).
+            constexpr int kTaken = EPI == EPI_GATED ? 2 : 1;
 #pragma unroll 1
-            for (int c = 0; c < (EPI == EPI_GATED ? kChunks / 2 : kChunks); c++) {
-                p.col0 = EPI == EPI_GATED ? (int64_t)at.n * kHalf + (half * (kChunks / 2) + c) * 32 : (int64_t)at.n * BN + half * kHalf + c * 32;
+            for (int c = 0; c < kChunks / kTaken; c++) {
+                p.col0 = ((int64_t)at.n * kBlocksN * 2 + half * kChunks) / kTaken * 32 + c * 32;
                 if (p.col0 >= g.cols) break;
-                if (EPI == EPI_GATED) {
-#pragma unroll 1
-                    for (int pass = 0; pass < 2; pass++) {  // 16 rows of both at a time fit the buffer
-                        __syncwarp();
-                        if (lane >> 4 == pass) {
+                if (g.wide && p.col0 + 32 <= g.cols) finish_wide<EPI>(g, acc[0], acc[kTaken - 1], p, s1, s2, buf, lane);
+                else finish_any<EPI>(g, acc[0], acc[kTaken - 1], p, s1, s2, buf, lane);
 #pragma unroll
-                            for (int u = 0; u < kChunks / 2; u++)
-                                if (c == u)
+                for (int u = 0; u < kChunks - kTaken; u++)
 #pragma unroll
-                                    for (int i = 0; i < 16; i++) {
-                                        const float* from = i < 8 ? acc[u] + 4 * i : acc[u + kChunks / 2] + 4 * (i - 8);
-                                        *reinterpret_cast<float4*>(buf + turned<EPI>(lane & 15, i)) = make_float4(from[0], from[1], from[2], from[3]);
-                                    }
-                        }
-                        __syncwarp();
-                        p.row0 = row0 + 16 * pass, p.rows = min(16, all_rows - 16 * pass);
-                        finish_piece<EPI, 16>(g, buf, p, s1, s2, lane);
-                    }
-                } else {
-                    __syncwarp();
-#pragma unroll
-                    for (int u = 0; u < kChunks; u++)
-                        if (c == u)
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                *reinterpret_cast<float4*>(buf + turned<EPI>(lane, i)) =
-                                    make_float4(acc[u][4 * i], acc[u][4 * i + 1], acc[u][4 * i + 2], acc[u][4 * i + 3]);
-                    __syncwarp();
-                    finish_piece<EPI, 32>(g, buf, p, s1, s2, lane);
-                }
+                    for (int i = 0; i < 32; i++) acc[u][i] = acc[u + kTaken][i];
             }
         }
         if (!ok && lane == 0) give_up(g, stop);
@@ -591,8 +604,9 @@ static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintpt
 
 cudaError_t launch_gemm(const GemmArgs& args, bool a_mn, bool b_mn, int pieces_b, Epilogue epi, int sm_count, cudaStream_t st) {
     GemmArgs g = args;
-    g.wide = g.cols % 4 == 0 && aligned(g.out, 16) && aligned(g.out2, 16) && aligned(g.bias, 16) && aligned(g.bias2, 16) && aligned(g.residual, 16) &&
-             aligned(g.save, 16) && aligned(g.save2, 16) && aligned(g.save8, 4) && aligned(g.save8_2, 4);
+    const bool ck = g.save8 || g.save8_2;
+    g.wide = g.cols % (ck ? 8 : 4) == 0 && aligned(g.out, 16) && aligned(g.out2, 16) && aligned(g.bias, 16) && aligned(g.bias2, 16) &&
+             aligned(g.residual, 16) && aligned(g.save, 16) && aligned(g.save2, 16) && aligned(g.save8, 8) && aligned(g.save8_2, 8);
     g.groups = ck8_groups(g.cols), g.exp_offset = ck8_exp_offset(g.rows, g.cols);
     if (epi == EPI_LINEAR) return launch_sized<2, false, false, EPI_LINEAR>(g, sm_count, st);
     if (epi == EPI_GATED) return launch_sized<2, false, false, EPI_GATED>(g, sm_count, st);
