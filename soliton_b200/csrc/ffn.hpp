@@ -12,11 +12,12 @@ enum Act : int { ACT_NONE = 0, ACT_GELU = 1, ACT_SILU = 2 };
 
 // ---------------------------------------------------------------- operand planes
 //
-// A plane holds a rows x cols matrix as fp16 pieces in blocks of 64 x 64. A block is the image of its values in shared
-// memory as the tensor cores read it: row r at byte 128 r, the row's eight 16-byte chunks at positions c ^ (r & 7) (the
+// A plane holds a rows x cols matrix as fp16 pieces in blocks of 64 x 64, each the image of its values in shared memory as
+// the tensor cores read it: groups of eight rows of 128 bytes, a row's eight 16-byte chunks at positions c ^ (row & 7) (the
 // 128-byte swizzle). The same image serves as 64 rows of a K-major operand tile and as 64 columns of an MN-major one, so
-// one plane feeds every product its matrix appears in, transposed or not. A block is `pieces` images of 8 KiB: the
-// value's upper 11 bits and, in a plane of two, the 11 bits that follow. Rows and columns beyond the matrix are zero.
+// one plane feeds every product its matrix appears in, transposed or not. In a plane of two pieces each group's upper 11
+// bits (hi, 1 KiB) are followed by the 11 bits after them (lo, 1 KiB). A block is one contiguous copy of 8 KiB a piece. Rows
+// and columns beyond the matrix are zero.
 constexpr int kBlock = 64;
 constexpr size_t kImageBytes = kBlock * kBlock * 2;
 constexpr int kAmaxParts = 296;     // partial maxima per tensor at the most, one per block of the maximum's kernel

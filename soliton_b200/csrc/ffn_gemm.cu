@@ -145,15 +145,17 @@ __device__ __forceinline__ void tmem_add16(unsigned addr, float* sum) {
     for (int i = 0; i < 16; i++) sum[i] += __uint_as_float(r[i]);
 }
 
-// Shared-memory descriptors of block images (128-byte swizzle, groups of eight 128-byte rows 1 KiB apart). K-major: a
-// row is 64 values along K, a step of 16 is 32 bytes. MN-major: a row is 64 values along M or N, eight rows (eight
-// steps along K) per group, the next 64 values one image further, a step of 16 is two groups.
-template <bool MN>
-__device__ __forceinline__ uint64_t descriptor(unsigned image) {
-    return (uint64_t)((image & 0x3ffff) >> 4) | (uint64_t)(MN ? kImageBytes >> 4 : 1) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// Shared-memory descriptors of blocks (128-byte swizzle; groups of eight 128-byte rows lie 1 KiB apart for each piece).
+// K-major: a row is 64 values along K, a step of 16 is 32 bytes. MN-major: a row is 64 values along M or N, eight rows
+// (eight steps along K) per group, the next 64 values one block further, a step of 16 is two groups.
+template <bool MN, int PIECES>
+__device__ __forceinline__ uint64_t descriptor(unsigned block) {
+    constexpr unsigned kGroupBytes = 1024 * PIECES, kBlockBytes = (unsigned)kImageBytes * PIECES;
+    return (uint64_t)((block & 0x3ffff) >> 4) | (uint64_t)(MN ? kBlockBytes >> 4 : 1) << 16 | (uint64_t)(kGroupBytes >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-template <bool MN>
-constexpr unsigned kStepBytes = MN ? 2048 : 32;
+template <bool MN, int PIECES>
+constexpr unsigned kStepBytes = MN ? 2048 * PIECES : 32;
+constexpr unsigned kLoBytes = 1024;  // from a group's hi to its lo
 
 // Blocks of B along N in a column of tiles: all, or at its end as many as exist -- an even number, so that a pair can halve
 // it (what is not there is never stored).
@@ -362,8 +364,8 @@ __device__ __forceinline__ Tile tile_at(int t, int m_tiles, int n_tiles) {
 template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
 __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs g) {
     constexpr int BN = 128 * CTAS, kBlocksN = BN / kBlock, kChunks = BN / 64;  // chunks of 32 columns a warp
-    constexpr int kOperandBytes = 2 * (int)kImageBytes;  // one piece of this block's 128 rows of A, or of its share of B
-    constexpr int kStageBytes = (2 + PB) * kOperandBytes;
+    constexpr unsigned kABlock = 2 * (unsigned)kImageBytes, kBBlock = PB * (unsigned)kImageBytes;
+    constexpr int kStageBytes = 2 * (kABlock + kBBlock);  // this block's 128 rows of A and its share of B
     constexpr int kStages = kRingBytes / kStageBytes < kMaxStages ? kRingBytes / kStageBytes : kMaxStages;
     extern __shared__ char raw[];
     char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -414,29 +416,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                         if (at.n * kBlocksN + i < g.b.mn_blocks) nb = j + 1;
                     }
                 }
-                const unsigned bytes = (unsigned)(na * 2 + nb * PB) * (unsigned)kImageBytes;
+                const unsigned bytes = (unsigned)na * kABlock + (unsigned)nb * kBBlock;
                 for (int kb = 0; kb < g.k_blocks; kb++, it++) {
                     const unsigned s = it % kStages, round = it / kStages;
                     if (!mbar_wait(empty + 8 * s, (round & 1) ^ 1, g.timeout_ns, stop)) {
                         ok = false;
                         break;
                     }
-                    const unsigned bar = full + 8 * s, at_a = ring_at + s * kStageBytes, at_b = at_a + 2 * kOperandBytes;
+                    const unsigned bar = full + 8 * s, at_a = ring_at + s * kStageBytes, at_b = at_a + 2 * kABlock;
                     mbar_expect(bar, bytes);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        if (i >= na) break;
-                        const char* src = g.a.plane + ((int64_t)(ma + i) * g.a.mn_stride + (int64_t)kb * g.a.k_stride) * (int64_t)(2 * kImageBytes);
-                        bulk_load(at_a + i * kImageBytes, src, kImageBytes, bar);
-                        bulk_load(at_a + kOperandBytes + i * kImageBytes, src + kImageBytes, kImageBytes, bar);
-                    }
+                    for (int i = 0; i < 2; i++)
+                        if (i < na)
+                            bulk_load(at_a + i * kABlock, g.a.plane + ((int64_t)(ma + i) * g.a.mn_stride + (int64_t)kb * g.a.k_stride) * (int64_t)kABlock, kABlock, bar);
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        if (j >= nb) break;
-                        const char* src = g.b.plane + (b_at[j] + (int64_t)kb * g.b.k_stride) * (int64_t)(PB * kImageBytes);
-                        bulk_load(at_b + j * kImageBytes, src, kImageBytes, bar);
-                        if (PB == 2) bulk_load(at_b + kOperandBytes + j * kImageBytes, src + kImageBytes, kImageBytes, bar);
-                    }
+                    for (int j = 0; j < 2; j++)
+                        if (j < nb) bulk_load(at_b + j * kBBlock, g.b.plane + (b_at[j] + (int64_t)kb * g.b.k_stride) * (int64_t)kBBlock, kBBlock, bar);
                 }
             }
             if (!ok) {  // nothing may still be on its way into this block's shared memory when it ends
@@ -470,15 +465,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                             break;
                         }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const unsigned at_a = ring_at + s * kStageBytes, at_b = at_a + 2 * kOperandBytes;
-                        const uint64_t a_hi = descriptor<AMN>(at_a), a_lo = descriptor<AMN>(at_a + kOperandBytes);
-                        const uint64_t b_hi = descriptor<BMN>(at_b), b_lo = descriptor<BMN>(at_b + kOperandBytes);
+                        const unsigned at_a = ring_at + s * kStageBytes, at_b = at_a + 2 * kABlock;
+                        const uint64_t a_hi = descriptor<AMN, 2>(at_a), b_hi = descriptor<BMN, PB>(at_b);
 #pragma unroll
                         for (int step = 0; step < kBlock / 16; step++) {
-                            const uint64_t da = (uint64_t)(step * kStepBytes<AMN> >> 4), db = (uint64_t)(step * kStepBytes<BMN> >> 4);
-                            mma_f16<CTAS>(d, a_lo + da, b_hi + db, idesc, !(kb == k0 && step == 0));
-                            mma_f16<CTAS>(d, a_hi + da, b_hi + db, idesc, 1);
-                            if (PB == 2) mma_f16<CTAS>(d, a_hi + da, b_lo + db, idesc, 1);
+                            const uint64_t da = a_hi + (step * kStepBytes<AMN, 2> >> 4), db = b_hi + (step * kStepBytes<BMN, PB> >> 4);
+                            mma_f16<CTAS>(d, da + (kLoBytes >> 4), db, idesc, !(kb == k0 && step == 0));
+                            mma_f16<CTAS>(d, da, db, idesc, 1);
+                            if (PB == 2) mma_f16<CTAS>(d, da, db + (kLoBytes >> 4), idesc, 1);
                         }
                         mma_commit<CTAS>(empty + 8 * s);
                     }

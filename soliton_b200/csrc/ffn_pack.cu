@@ -128,11 +128,13 @@ __device__ __forceinline__ void split8(const Eight& x, float scale, uint4& hi, u
     hi = make_uint4(h[0], h[1], h[2], h[3]), lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-__device__ __forceinline__ void store_pieces(char* block, int pieces, int at, const Eight& x, float scale) {
+// Row r, eight columns `chunk` of a block.
+__device__ __forceinline__ void store_pieces(char* block, int pieces, int r, int chunk, const Eight& x, float scale) {
     uint4 hi, lo;
     split8(x, scale, hi, lo);
-    *reinterpret_cast<uint4*>(block + at) = hi;
-    if (pieces == 2) *reinterpret_cast<uint4*>(block + kImageBytes + at) = lo;
+    char* at = block + (r >> 3) * (1024 * pieces) + (r & 7) * 128 + ((chunk ^ (r & 7)) << 4);
+    *reinterpret_cast<uint4*>(at) = hi;
+    if (pieces == 2) *reinterpret_cast<uint4*>(at + 1024) = lo;
 }
 
 // Column sums over a block's 64 rows: a thread holds two rows' eight columns; four rows meet in a warp, then the eight
@@ -186,7 +188,7 @@ __device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scal
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int r = row_in + 32 * h, at = r * 128 + ((chunk ^ (r & 7)) << 4);
+        const int r = row_in + 32 * h;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (KIND == PACK_ACT) x[h].v[i] *= act_grad(j.act, y[h].v[i]);
@@ -196,8 +198,8 @@ __device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scal
                 y[h].v[i] = d * act_of(j.act, gate);
             }
         }
-        store_pieces(block, KIND == PACK_CK8 ? 1 : 2, at, x[h], scale);
-        if (KIND == PACK_GATED) store_pieces(block + (int64_t)j.second * (int64_t)(2 * kImageBytes), 2, at, y[h], scale);
+        store_pieces(block, KIND == PACK_CK8 ? 1 : 2, r, chunk, x[h], scale);
+        if (KIND == PACK_GATED) store_pieces(block + (int64_t)j.second * (int64_t)(2 * kImageBytes), 2, r, chunk, y[h], scale);
     }
     if (KIND != PACK_CK8 && j.colsum) block_colsum(x, s_sum, j.colsum + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
     if (KIND == PACK_GATED && j.colsum2) block_colsum(y, s_sum, j.colsum2 + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
