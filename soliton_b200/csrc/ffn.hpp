@@ -66,6 +66,24 @@ struct PackArgs {
     int jobs, units;
     AmaxArgs amax;
     int* exps;                      // out: values of plane i were multiplied by 2^(15 - exps[i])
+    int* counters;                  // to be zeroed for the products that follow
+    int n_counters;
+};
+// A forward pass's planes: every row has its own scale, so one read of the tensor is enough.
+struct RowJob {
+    const float* a;
+    int64_t rows, cols;
+    int col_blocks;
+    char* plane;                    // two pieces
+    float* factor;                  // out, whole blocks of rows: what undoes a row's scaling, times 2^-30 with `is_a`
+    int is_a;
+    int first_group;                // groups of eight rows of the jobs before this one
+};
+struct RowArgs {
+    RowJob job[3];
+    int jobs, groups;
+    int* counters;
+    int n_counters;
 };
 
 // ---------------------------------------------------------------- products
@@ -75,14 +93,18 @@ struct Operand {
     const char* plane;
     int64_t mn_stride, k_stride;    // in blocks
     int mn_blocks;                  // blocks along M or N that exist
-    int exp_id;
+    int exp_id;                     // EPI_STORE: the plane's exponent
 };
 enum Epilogue : int { EPI_STORE = 0, EPI_LINEAR = 1, EPI_GATED = 2 };
 struct GemmArgs {
     Operand a, b;
     int k_blocks;
     int m_tiles, n_tiles;           // set by launch_gemm
-    const int* exps;
+    const int* exps;                // EPI_STORE
+    const float *row_factor, *col_factor, *col_factor2;  // otherwise: of the rows of A and of B (EPI_GATED: of its two weights)
+    int whole, slices;              // set by launch_gemm: tiles done by one team, and into how many slices along K the others are cut
+    float* partial;                 // sums of those slices (gemm_plan's partial_bytes), and a counter per warp of their tiles, zeroed
+    int* counters;
     int* status;                    // sticky status word (host memory), or null
     unsigned long long timeout_ns;  // bound of every wait
     int64_t rows, cols;             // of the output (EPI_GATED: cols of each of the two)
@@ -97,6 +119,17 @@ struct GemmArgs {
     int wide;                       // set by launch_gemm: rows and pointers allow 16-byte accesses (8-byte for checkpoints)
 };
 
+// How a product is cut, from its sizes in blocks alone (for 148 SMs), so that a dry run knows the scratch.
+struct GemmPlan {
+    int ctas;                       // 1: tiles of 128 x 128 by single blocks; 2: 256 x 256 by pairs
+    int m_tiles, n_tiles;
+    int whole, slices;
+    size_t partial_bytes;
+    int counters;
+};
+GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks);
+
+cudaError_t launch_rows(const RowArgs& a, cudaStream_t st);
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
 cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st);
 // out[j] = the sum over `parts` of the block rows' column sums, in order
@@ -117,6 +150,23 @@ cudaError_t launch_ck8_load(const char* ck, float* x, int64_t rows, int64_t cols
 cudaError_t launch_ck8_gelu_bwd(const char* ck, const float* dy, float* dx, int64_t rows, int64_t cols, cudaStream_t st);
 
 #ifdef __CUDACC__
+// A launch that may begin while the kernel before it drains; what it does before stream_wait() must not touch memory that
+// kernel writes or reads.
+template <class... Params, class... Args>
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...);
+}
+__device__ __forceinline__ void stream_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void stream_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // The exponent byte of a group whose largest magnitude has these bits (sign cleared): the smallest e >= -126 with
 // 127 * 2^e >= the magnitude, plus 127; 255 when the group holds an infinity or a NaN. In a normal magnitude
 // 1.f * 2^p, 127 * 2^(p - 6) = 1.984375 * 2^p suffices up to f = 0.984375 and 2^(p - 5) is needed beyond.

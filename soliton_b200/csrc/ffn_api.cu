@@ -42,22 +42,41 @@ struct Carver {
 struct Scratch {
     int* exps;
     float *parts, *colsum, *colsum2;
+    float *row_factor, *col_factor, *col_factor2;
     char *y, *x, *w;        // planes: the gradient of the pre-activations, the input, the weights
+    float* partial;
+    int* counters;          // of the first product, then of the second
+    int n_counters;
 };
-// width: features out, of both weights side by side for the gated block (each padded to whole blocks)
+// weights: one, or the gated block's two side by side (each padded to whole blocks)
 size_t carve(Scratch& s, void* base, int64_t m, int64_t n, int64_t k, int weights, bool backward) {
     Carver c{static_cast<char*>(base)};
+    s = Scratch{};
+    const int64_t mb = blocks_of(m), nb = blocks_of(n), kb = blocks_of(k);
     const size_t block = 2 * kImageBytes;
-    s.exps = reinterpret_cast<int*>(c.take(kMaxPlanes * sizeof(int)));
-    s.parts = reinterpret_cast<float*>(c.take(kMaxSlots * kAmaxParts * sizeof(float)));
-    s.x = c.take((size_t)(blocks_of(m) * blocks_of(k)) * block);
-    s.w = c.take((size_t)(weights * blocks_of(n) * blocks_of(k)) * block);
-    s.y = nullptr, s.colsum = s.colsum2 = nullptr;
+    size_t partial;
+    s.x = c.take((size_t)(mb * kb) * block);
+    s.w = c.take((size_t)(weights * nb * kb) * block);
     if (backward) {
-        s.y = c.take((size_t)(weights * blocks_of(m) * blocks_of(n)) * block);
-        s.colsum = reinterpret_cast<float*>(c.take((size_t)(blocks_of(m) * n) * sizeof(float)));
-        s.colsum2 = weights == 2 ? reinterpret_cast<float*>(c.take((size_t)(blocks_of(m) * n) * sizeof(float))) : nullptr;
+        const GemmPlan dx = gemm_plan(mb, kb, weights * nb), dw = gemm_plan(weights * nb, kb, mb), half = gemm_plan(nb, kb, mb);
+        const int dw_counters = dw.counters > half.counters ? dw.counters : half.counters;
+        s.y = c.take((size_t)(weights * mb * nb) * block);
+        s.exps = reinterpret_cast<int*>(c.take(kMaxPlanes * sizeof(int)));
+        s.parts = reinterpret_cast<float*>(c.take(kMaxSlots * kAmaxParts * sizeof(float)));
+        s.colsum = reinterpret_cast<float*>(c.take((size_t)(mb * n) * sizeof(float)));
+        s.colsum2 = weights == 2 ? reinterpret_cast<float*>(c.take((size_t)(mb * n) * sizeof(float))) : nullptr;
+        s.n_counters = dx.counters + dw_counters;
+        partial = dx.partial_bytes > dw.partial_bytes ? dx.partial_bytes : dw.partial_bytes;
+        if (half.partial_bytes > partial) partial = half.partial_bytes;  // one of the gated pair's weights alone
+    } else {
+        const GemmPlan p = gemm_plan(mb, weights * nb, kb);
+        s.row_factor = reinterpret_cast<float*>(c.take((size_t)(mb * kBlock) * sizeof(float)));
+        s.col_factor = reinterpret_cast<float*>(c.take((size_t)(nb * kBlock) * sizeof(float)));
+        s.col_factor2 = weights == 2 ? reinterpret_cast<float*>(c.take((size_t)(nb * kBlock) * sizeof(float))) : nullptr;
+        s.n_counters = p.counters, partial = p.partial_bytes;
     }
+    s.counters = reinterpret_cast<int*>(c.take((size_t)s.n_counters * sizeof(int)));
+    s.partial = reinterpret_cast<float*>(c.take(partial));
     return c.used;
 }
 
@@ -115,7 +134,7 @@ int refuse(int code) {
 
 struct Planner {
     PackArgs p{};
-    explicit Planner(const Scratch& s) { p.amax.parts = s.parts, p.exps = s.exps; }
+    explicit Planner(const Scratch& s) { p.amax.parts = s.parts, p.exps = s.exps, p.counters = s.counters, p.n_counters = s.n_counters; }
     int slot(const float* x, const void* ck, int64_t rows, int64_t cols) {
         AmaxSlot& t = p.amax.slot[p.amax.slots];
         t.is_ck8 = x == nullptr;
@@ -146,9 +165,22 @@ struct Planner {
     }
 };
 
+// Planes of a forward pass.
+struct RowPlanner {
+    RowArgs r{};
+    explicit RowPlanner(const Scratch& s) { r.counters = s.counters, r.n_counters = s.n_counters; }
+    void matrix(const float* x, int64_t rows, int64_t cols, char* plane, float* factor, bool is_a) {
+        RowJob& j = r.job[r.jobs++];
+        j.a = x, j.rows = rows, j.cols = cols, j.col_blocks = (int)blocks_of(cols), j.plane = plane, j.factor = factor, j.is_a = is_a;
+        j.first_group = r.groups;
+        r.groups += (int)blocks_of(rows) * (kBlock / 8);
+    }
+};
+
 GemmArgs product(const Op& op, const Scratch& s) {
     GemmArgs g{};
-    g.exps = s.exps, g.status = op.status(), g.timeout_ns = op.timeout_ns(), g.split = INT64_MAX;
+    g.exps = s.exps, g.row_factor = s.row_factor, g.col_factor = s.col_factor, g.col_factor2 = s.col_factor2;
+    g.partial = s.partial, g.counters = s.counters, g.status = op.status(), g.timeout_ns = op.timeout_ns(), g.split = INT64_MAX;
     return g;
 }
 // A plane whose block rows run along M or N (K-major), or along K (MN-major).
@@ -167,11 +199,9 @@ int run_linear(const float* x, const float* w, const float* bias, const float* r
     const size_t bytes = carve(s, scratch, m, n, k, 1, false);
     op.reads(x, 4 * m * k), op.reads(w, 4 * n * k), op.reads(bias, 4 * n), op.reads(residual, 4 * m * n);
     op.writes(y, 4 * m * n), op.writes(pre, 4 * m * n), op.writes(pre8, pre8 ? ck8_bytes(m, n) : 0), op.writes(scratch, (int64_t)bytes);
-    Planner p(s);
-    p.slot(x, nullptr, m, k), p.slot(w, nullptr, n, k);
-    p.matrix(x, nullptr, m, k, s.x, PLANE_X, 1);
-    p.matrix(w, nullptr, n, k, s.w, PLANE_W, 2);
-    p.launch(op);
+    RowPlanner p(s);
+    p.matrix(x, m, k, s.x, s.row_factor, true), p.matrix(w, n, k, s.w, s.col_factor, false);
+    op.launched(launch_rows(p.r, 0));
     GemmArgs g = product(op, s);
     const int64_t kb = blocks_of(k);
     g.a = k_major(s.x, blocks_of(m), kb, PLANE_X), g.b = k_major(s.w, blocks_of(n), kb, PLANE_W);
@@ -191,12 +221,10 @@ int run_gated(const float* x, const float* wg, const float* wu, const float* bg,
     op.writes(h, 4 * m * f), op.writes(gate, 4 * m * f), op.writes(up, 4 * m * f), op.writes(scratch, (int64_t)bytes);
     op.writes(gate8, gate8 ? ck8_bytes(m, f) : 0), op.writes(up8, up8 ? ck8_bytes(m, f) : 0);
     const int64_t kb = blocks_of(k), fb = blocks_of(f);
-    Planner p(s);
-    p.slot(x, nullptr, m, k), p.slot(wg, nullptr, f, k), p.slot(wu, nullptr, f, k);
-    p.matrix(x, nullptr, m, k, s.x, PLANE_X, 1);
-    p.matrix(wg, nullptr, f, k, s.w, PLANE_W, 6);
-    p.matrix(wu, nullptr, f, k, s.w + fb * kb * (int64_t)(2 * kImageBytes), PLANE_W, 6);
-    p.launch(op);
+    RowPlanner p(s);
+    p.matrix(x, m, k, s.x, s.row_factor, true), p.matrix(wg, f, k, s.w, s.col_factor, false);
+    p.matrix(wu, f, k, s.w + fb * kb * (int64_t)(2 * kImageBytes), s.col_factor2, false);
+    op.launched(launch_rows(p.r, 0));
     GemmArgs g = product(op, s);
     g.a = k_major(s.x, blocks_of(m), kb, PLANE_X), g.b = k_major(s.w, 2 * fb, kb, PLANE_W);
     g.k_blocks = (int)kb, g.rows = m, g.cols = f, g.act = act, g.gate_blocks = (int)fb;
@@ -220,6 +248,7 @@ void gradients(Op& op, const Scratch& s, bool x_ck8, float* dx, float* dw, float
         const bool both = dw && dw2;
         const char* y = s.y + (halves == 2 && !dw ? nb * (int64_t)(2 * kImageBytes) : 0);
         GemmArgs g = product(op, s);
+        g.counters += gemm_plan(mb, kb, width).counters;  // behind dx's
         g.a = mn_major(y, both ? width : nb, width, PLANE_Y), g.b = mn_major(s.x, kb, kb, PLANE_X);
         g.k_blocks = (int)mb, g.rows = n, g.cols = k, g.out = dw ? dw : dw2;
         if (both) g.split = nb * kBlock, g.out2 = dw2;

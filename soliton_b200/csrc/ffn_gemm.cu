@@ -14,6 +14,8 @@
 // The epilogue works on the accumulator's own arrangement, a row per lane and 32 columns at a time (one group of a
 // checkpoint), and turns pieces of 32 x 32 through shared memory to store them in whole lines.
 //
+// Forward, the rows of both operands have their own scales, which the epilogue undoes; backward the whole planes'.
+//
 // Every wait is bounded: a block whose wait runs out records ST_TIMEOUT_PRODUCT, waits (bounded) for its copies and
 // products in flight, frees its tensor memory and returns.
 #include "dp_types.h"
@@ -32,6 +34,7 @@ constexpr int kTurnFloats = 32 * 32;                        // one warp's turnin
 constexpr int kSmemBytes = kRingBytes + kEpiWarps * kTurnFloats * 4 + 256 + 1024;
 constexpr int kSegment = 4, kFirstSegments = 6;             // k-blocks per accumulator segment; in a tile's first two
 constexpr int kMaxStages = 4;
+constexpr int kPlanSMs = 148;                               // how products are cut must not depend on the device
 constexpr int kGroupM = 8;                                  // row tiles that blocks walk side by side (reuse in L2)
 
 __device__ __forceinline__ unsigned smem_addr(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -233,12 +236,15 @@ __device__ __forceinline__ void keep_wide(const float (&v)[32], const Piece& p, 
         ck[g.exp_offset + (p.row0 + lane) * g.groups + p.col0 / kGroup] = (char)byte;
     }
 }
-__device__ __forceinline__ void scale_row(float (&v)[32], float s1, float s2, const float* bias) {
+// Undoes the operands' scaling, which cannot overflow before the result does: the row's factor is 2^-30 of its magnitude.
+// `col` and `bias`: of the 32 columns.
+__device__ __forceinline__ void scale_row(float (&v)[32], float row, const float* col, const float* bias) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(col + i);
         const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        v[i] = fmaf(v[i] * s1, s2, b.x), v[i + 1] = fmaf(v[i + 1] * s1, s2, b.y);
-        v[i + 2] = fmaf(v[i + 2] * s1, s2, b.z), v[i + 3] = fmaf(v[i + 3] * s1, s2, b.w);
+        v[i] = fmaf(v[i] * row, c.x, b.x), v[i + 1] = fmaf(v[i + 1] * row, c.y, b.y);
+        v[i + 2] = fmaf(v[i + 2] * row, c.z, b.z), v[i + 3] = fmaf(v[i + 3] * row, c.w, b.w);
     }
 }
 template <int ACT>
@@ -262,12 +268,15 @@ template <int EPI>
 __device__ __forceinline__ void finish_wide(const GemmArgs& g, float (&v)[32], float (&w)[32], const Piece& p, float s1, float s2, float* buf, int lane) {
     const bool second = EPI == EPI_STORE && p.row0 >= g.split;
     const int64_t at = (p.row0 - (second ? g.split : 0)) * g.cols + p.col0;
-    scale_row(v, s1, s2, EPI != EPI_STORE && g.bias ? g.bias + p.col0 : nullptr);
-    if (EPI != EPI_STORE) {
+    if (EPI == EPI_STORE) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = v[i] * s1 * s2;
+    } else {
+        scale_row(v, s1, g.col_factor + p.col0, g.bias ? g.bias + p.col0 : nullptr);
         keep_wide(v, p, at, g, g.save, g.save8, buf, lane);
         act_row(g.act, v);
         if (EPI == EPI_GATED) {
-            scale_row(w, s1, s2, g.bias2 ? g.bias2 + p.col0 : nullptr);
+            scale_row(w, s1, g.col_factor2 + p.col0, g.bias2 ? g.bias2 + p.col0 : nullptr);
             keep_wide(w, p, at, g, g.save2, g.save8_2, buf, lane);
 #pragma unroll
             for (int i = 0; i < 32; i++) v[i] *= w[i];
@@ -305,19 +314,23 @@ __device__ __forceinline__ void finish_any(const GemmArgs& g, float (&v)[32], fl
     const int64_t row = p.row0 - (second ? g.split : 0), col = p.col0 + lane, at = row * g.cols + col;
     const bool ok = col < g.cols;
     float* out = (second ? g.out2 : g.out) + at;
-    turn(v, buf, lane);
-    const float bias = EPI != EPI_STORE && g.bias && ok ? __ldg(g.bias + col) : 0.0f;
 #pragma unroll
-    for (int r = 0; r < 32; r++) v[r] = fmaf(v[r] * s1, s2, bias);
+    for (int i = 0; i < 32; i++) v[i] *= s1;
+    turn(v, buf, lane);
+    const float bias = EPI != EPI_STORE && g.bias && ok ? __ldg(g.bias + col) : 0.0f, by = EPI == EPI_STORE ? s2 : g.col_factor[col];
+#pragma unroll
+    for (int r = 0; r < 32; r++) v[r] = fmaf(v[r], by, bias);
     if (EPI != EPI_STORE) {
         const int64_t group = row * g.groups + p.col0 / kGroup;
         keep_column(v, p.rows, ok, at, group, g, g.save, g.save8, lane);
         act_row(g.act, v);
         if (EPI == EPI_GATED) {
-            turn(w, buf, lane);
-            const float bias2 = g.bias2 && ok ? __ldg(g.bias2 + col) : 0.0f;
 #pragma unroll
-            for (int r = 0; r < 32; r++) w[r] = fmaf(w[r] * s1, s2, bias2);
+            for (int i = 0; i < 32; i++) w[i] *= s1;
+            turn(w, buf, lane);
+            const float bias2 = g.bias2 && ok ? __ldg(g.bias2 + col) : 0.0f, by2 = g.col_factor2[col];
+#pragma unroll
+            for (int r = 0; r < 32; r++) w[r] = fmaf(w[r], by2, bias2);
             keep_column(w, p.rows, ok, at, group, g, g.save2, g.save8_2, lane);
 #pragma unroll
             for (int r = 0; r < 32; r++) v[r] *= w[r];
@@ -347,13 +360,63 @@ __device__ __forceinline__ int segment_end(int k0, int k_blocks) {
     return min(k0 + (k0 < 2 * kFirstSegments ? kFirstSegments : kSegment), k_blocks);
 }
 
-struct Tile {
-    int m, n;
+// What a team takes up at a time: a tile, or a slice of one along K. Tiles that would leave most teams idle in the last
+// round are cut so that every team has a part.
+struct Unit {
+    int m, n, k0, k1, slice;        // slice: of all, -1 for a whole tile
 };
-__device__ __forceinline__ Tile tile_at(int t, int m_tiles, int n_tiles) {
-    const int per_group = kGroupM * n_tiles, group = t / per_group, in_group = t - group * per_group;
-    const int first = group * kGroupM, height = min(kGroupM, m_tiles - first);
-    return Tile{first + in_group % height, in_group / height};
+__device__ __forceinline__ int units_of(const GemmArgs& g) { return g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices; }
+__device__ __forceinline__ Unit unit_at(int u, const GemmArgs& g) {
+    Unit r;
+    int t = u;
+    r.slice = -1, r.k0 = 0, r.k1 = g.k_blocks;
+    if (u >= g.whole) {
+        r.slice = u - g.whole;
+        const int s = r.slice % g.slices;
+        t = g.whole + r.slice / g.slices;
+        r.k0 = (int)((int64_t)g.k_blocks * s / g.slices), r.k1 = (int)((int64_t)g.k_blocks * (s + 1) / g.slices);
+    }
+    const int per_group = kGroupM * g.n_tiles, group = t / per_group, in_group = t - group * per_group;
+    const int first = group * kGroupM, height = min(kGroupM, g.m_tiles - first);
+    r.m = first + in_group % height, r.n = in_group / height;
+    return r;
+}
+
+// A warp's sums over one slice of a tile go to memory; the warp that comes last adds up all slices, in their order, and has
+// the tile (true). Nobody waits. `who` of `warps`: the part of the tile.
+template <int CHUNKS>
+__device__ __forceinline__ bool add_slices(const GemmArgs& g, float (&acc)[CHUNKS][32], int slice, int warps, int who, int lane) {
+    constexpr int kFloats = CHUNKS * 32 * 32;
+    const auto place = [&](int s) { return reinterpret_cast<float4*>(g.partial) + ((int64_t)s * warps + who) * (kFloats / 4) + lane; };
+    float4* mine = place(slice);
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) __stcg(mine + (c * 8 + i) * 32, make_float4(acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]));
+    __threadfence();
+    __syncwarp();
+    int before = 0;
+    if (lane == 0) before = atomicAdd(g.counters + (slice / g.slices) * warps + who, 1);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    if (before != g.slices - 1) return false;
+    __threadfence();
+    const int first = slice - slice % g.slices;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+        for (int i = 0; i < 32; i++) acc[c][i] = 0.0f;
+#pragma unroll 1
+    for (int s = 0; s < g.slices; s++) {
+        const float4* from = place(first + s);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float4 v = __ldcg(from + (c * 8 + i) * 32);
+                acc[c][4 * i] += v.x, acc[c][4 * i + 1] += v.y, acc[c][4 * i + 2] += v.z, acc[c][4 * i + 3] += v.w;
+            }
+    }
+    return true;
 }
 
 // CTAS = 1: a block per tile of 128 x 128. CTAS = 2: a pair of blocks (a cluster) per tile of 256 x 256: each holds 128 rows of A
@@ -389,19 +452,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) tmem_alloc<CTAS>(smem_addr(words + 1));
+    stream_next();
+    stream_wait();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     team_sync<CTAS>();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = *reinterpret_cast<volatile unsigned*>(words + 1);
-    const int tiles = g.m_tiles * g.n_tiles;
+    const int units = units_of(g);
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
         if (warp == 0 && lane == 0) {
             unsigned it = 0;
             bool ok = true;
-            for (int t = team; ok && t < tiles; t += teams) {
-                const Tile at = tile_at(t, g.m_tiles, g.n_tiles);
+            for (int t = team; ok && t < units; t += teams) {
+                const Unit at = unit_at(t, g);
                 const int ma = (at.m * CTAS + rank) * 2, na = max(0, min(2, g.a.mn_blocks - ma));
                 const int width = blocks_wide<CTAS, EPI>(g, at.n), share = width / CTAS;  // blocks of B: the tile's and this block's
                 int64_t b_at[2];
@@ -417,7 +482,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                     }
                 }
                 const unsigned bytes = (unsigned)na * kABlock + (unsigned)nb * kBBlock;
-                for (int kb = 0; kb < g.k_blocks; kb++, it++) {
+                for (int kb = at.k0; kb < at.k1; kb++, it++) {
                     const unsigned s = it % kStages, round = it / kStages;
                     if (!mbar_wait(empty + 8 * s, (round & 1) ^ 1, g.timeout_ns, stop)) {
                         ok = false;
@@ -445,12 +510,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         if (warp == 1 && lane == 0 && rank == 0) {
             unsigned it = 0, seg = 0;
             bool ok = true;
-            for (int t = team; ok && t < tiles; t += teams) {
-                const Tile at = tile_at(t, g.m_tiles, g.n_tiles);
+            for (int t = team; ok && t < units; t += teams) {
+                const Unit at = unit_at(t, g);
                 const unsigned idesc = 1u << 4 | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u) | (unsigned)(blocks_wide<CTAS, EPI>(g, at.n) * kBlock >> 3) << 17 |
                                        (unsigned)(BM * CTAS >> 4) << 24;
-                for (int k0 = 0, k1; ok && k0 < g.k_blocks; k0 = k1, seg++) {
-                    k1 = segment_end(k0, g.k_blocks);
+                const int k_blocks = at.k1 - at.k0;
+                for (int k0 = 0, k1; ok && k0 < k_blocks; k0 = k1, seg++) {
+                    k1 = segment_end(k0, k_blocks);
                     const unsigned buf = seg & 1, d = tmem + buf * BN;
                     if (!mbar_wait<CTAS == 2>(tempty + 8 * buf, ((seg >> 1) & 1) ^ 1, g.timeout_ns, stop)) {
                         ok = false;
@@ -487,7 +553,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         }
         if (CTAS == 2 && warp == 1 && lane == 0 && rank == 1) {
             const unsigned there = remote(peer_full, 0);
-            const int rounds = tiles > team ? ((tiles - team - 1) / teams + 1) * g.k_blocks : 0;
+            int rounds = 0;
+            for (int t = team; t < units; t += teams) {
+                const Unit at = unit_at(t, g);
+                rounds += at.k1 - at.k0;
+            }
             for (int it = 0; it < rounds; it++) {
                 const unsigned s = (unsigned)it % kStages;
                 if (!mbar_wait(full + 8 * s, ((unsigned)it / kStages) & 1, g.timeout_ns, stop)) {
@@ -502,12 +572,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         const int q = warp & 3, half = (warp >> 2) - 1;  // a warp reads the 32 rows of tensor memory that its number mod 4 gives
         float* buf = turn + (warp - 4) * kTurnFloats;
-        const int e = g.exps[g.a.exp_id] + g.exps[g.b.exp_id] - 30;  // undo both planes' scaling, in two steps that cannot overflow early
-        const float s1 = exp2f((float)(e / 2)), s2 = exp2f((float)(e - e / 2));
+        float s1 = 0.0f, s2 = 0.0f;
+        if (EPI == EPI_STORE) {  // undo both planes' scaling, in two steps that cannot overflow before the result does
+            const int e = g.exps[g.a.exp_id] + g.exps[g.b.exp_id] - 30;
+            s1 = exp2f((float)(e / 2)), s2 = exp2f((float)(e - e / 2));
+        }
         unsigned seg = 0;
         bool ok = true;
-        for (int t = team; ok && t < tiles; t += teams) {
-            const Tile at = tile_at(t, g.m_tiles, g.n_tiles);
+        for (int t = team; ok && t < units; t += teams) {
+            const Unit at = unit_at(t, g);
             float acc[kChunks][32];
 #pragma unroll
             for (int c = 0; c < kChunks; c++)
@@ -519,7 +592,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                     for (int64_t c = col; c < min(col + kChunks * 32, g.cols); c += 32)
                         asm volatile("prefetch.global.L2 [%0];" ::"l"(g.residual + row * g.cols + c));
             }
-            for (int k0 = 0; k0 < g.k_blocks; k0 = segment_end(k0, g.k_blocks), seg++) {
+            const int k_blocks = at.k1 - at.k0;
+            for (int k0 = 0; k0 < k_blocks; k0 = segment_end(k0, k_blocks), seg++) {
                 const unsigned b = seg & 1;
                 ok = __all_sync(0xffffffffu, mbar_wait(tfull + 8 * b, (seg >> 1) & 1, g.timeout_ns, stop));
                 if (!ok) break;
@@ -537,12 +611,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                 }
             }
             if (!ok) break;
+            if (at.slice >= 0 && !add_slices(g, acc, at.slice, CTAS * kEpiWarps, rank * kEpiWarps + warp - 4, lane)) continue;
             Piece p;
             p.row0 = (int64_t)(at.m * CTAS + rank) * BM + q * 32;
             int64_t left = g.rows - p.row0;
             if (EPI == EPI_STORE && p.row0 >= g.split) left += g.split;
             p.rows = left < 0 ? 0 : left < 32 ? (int)left : 32;
             if (p.rows == 0) continue;
+            if (EPI != EPI_STORE) s1 = g.row_factor[p.row0 + lane];  // whole blocks of factors exist
             // In place and in a loop that moves the next chunk up: registers are short, and so should the code be, which runs
             // once per tile and is bound by fetching it when it is long (150 k cycles a tile for four chunks in a row).
             constexpr int kTaken = EPI == EPI_GATED ? 2 : 1;
@@ -569,29 +645,53 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     }
 }
 
+// ---------------------------------------------------------------- how a product is cut
+
+// Estimated cycles of a way of cutting: rounds of whole tiles, then the slices. A k-block takes a pair 1,750 cycles, bound by
+// what the L2 delivers, and a single block, which fetches as much for half the work, the same when most SMs run, 1,100
+// when few do; a tile's first fetches and what of its epilogue nothing covers 9,000 (6,000 single); a slice's sums are
+// written once and read once, 3,000 each (1,500).
+static double cut_cost(int ctas, int64_t tiles, int64_t k_blocks, int64_t slices) {
+    const int64_t teams = kPlanSMs / ctas, rounds = tiles / teams, rest = tiles % teams;
+    const int64_t busy = rounds > 0 ? kPlanSMs : rest * slices * ctas;
+    const double block = ctas == 2 || busy > 100 ? 1750 : 1100, tile = ctas == 2 ? 9000 : 6000, slice = ctas == 2 ? 3000 : 1500;
+    double t = (double)rounds * (block * (double)k_blocks + tile);
+    if (rest) t += block * (double)((k_blocks + slices - 1) / slices) + tile + (slices > 1 ? slice * (double)(1 + slices) : 0.0);
+    return t;
+}
+
+GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks) {
+    GemmPlan best{};
+    double least = 0;
+    for (int ctas = 1; ctas <= 2; ctas++) {
+        const int64_t mt = (m_blocks + 2 * ctas - 1) / (2 * ctas), nt = (n_blocks + 2 * ctas - 1) / (2 * ctas), tiles = mt * nt;
+        const int64_t teams = kPlanSMs / ctas, rest = tiles % teams;
+        const int64_t most = rest ? teams / rest : 1;
+        for (int64_t s = 1; s <= most && s <= k_blocks && s <= 16; s++) {
+            const double t = cut_cost(ctas, tiles, k_blocks, s);
+            if (best.ctas && t >= least) continue;
+            least = t;
+            best.ctas = ctas, best.m_tiles = (int)mt, best.n_tiles = (int)nt;
+            best.whole = (int)(s > 1 ? tiles - rest : tiles), best.slices = (int)s;
+            best.counters = s > 1 ? (int)rest * ctas * kEpiWarps : 0;
+            best.partial_bytes = s > 1 ? (size_t)(rest * s) * (size_t)ctas * 128 * (128 * (size_t)ctas) * sizeof(float) : 0;
+        }
+    }
+    return best;
+}
+
 template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
-static cudaError_t launch_one(GemmArgs g, int sm_count, cudaStream_t st) {
+static cudaError_t launch_one(const GemmArgs& g, int sm_count, cudaStream_t st) {
     static const cudaError_t ready = cudaFuncSetAttribute(k_gemm<CTAS, PB, AMN, BMN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (ready != cudaSuccess) return ready;
-    const int width = EPI == EPI_GATED ? 2 * g.gate_blocks : g.b.mn_blocks;
-    g.m_tiles = (g.a.mn_blocks + 2 * CTAS - 1) / (2 * CTAS), g.n_tiles = (width + 2 * CTAS - 1) / (2 * CTAS);
-    const int tiles = g.m_tiles * g.n_tiles, teams = sm_count / CTAS;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(CTAS * (tiles < teams ? tiles : teams))), cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = kSmemBytes, cfg.stream = st;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = CTAS, cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    cfg.attrs = &cluster, cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_gemm<CTAS, PB, AMN, BMN, EPI>, g);
+    const int units = g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices, teams = sm_count / CTAS;
+    return launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
 }
 template <int PB, bool AMN, bool BMN, int EPI>
-static cudaError_t launch_sized(const GemmArgs& g, int sm_count, cudaStream_t st) {
-    // Single blocks as long as their smaller tiles all run at once: a pair's tile would take longer. Beyond that the
-    // pairs' smaller traffic decides.
-    const int64_t width = EPI == EPI_GATED ? 2 * (int64_t)g.gate_blocks : g.b.mn_blocks;
-    const int64_t singles = ((g.a.mn_blocks + 1) / 2) * ((width + 1) / 2);
-    return singles <= sm_count ? launch_one<1, PB, AMN, BMN, EPI>(g, sm_count, st) : launch_one<2, PB, AMN, BMN, EPI>(g, sm_count, st);
+static cudaError_t launch_sized(GemmArgs& g, int sm_count, cudaStream_t st) {
+    const GemmPlan p = gemm_plan(g.a.mn_blocks, EPI == EPI_GATED ? 2 * (int64_t)g.gate_blocks : g.b.mn_blocks, g.k_blocks);
+    g.m_tiles = p.m_tiles, g.n_tiles = p.n_tiles, g.whole = p.whole, g.slices = p.slices;
+    return p.ctas == 1 ? launch_one<1, PB, AMN, BMN, EPI>(g, sm_count, st) : launch_one<2, PB, AMN, BMN, EPI>(g, sm_count, st);
 }
 
 static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

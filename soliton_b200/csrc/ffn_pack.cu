@@ -1,16 +1,18 @@
 // Operand planes for the products (ffn.hpp): the largest magnitude of each tensor, then fp32 values (or a checkpoint's,
 // or the gradient that an activation hands back) as scaled fp16 pieces in the tensor cores' block layout.
 //
-// The tensor cores have no fp32. A value times a power of two, t = x * 2^(15 - E) with |x| < 2^E for the whole tensor,
+// The tensor cores have no fp32. A value times a power of two, t = x * 2^(15 - E) with |x| < 2^E,
 // is cut into hi = fp16(t) and lo = fp16(t - hi): 22 bits of x wherever |x| > 2^(E - 17), and an absolute error of
 // 2^(E - 40) below that. A product of two such values takes three fp16 products, hi*hi + hi*lo + lo*hi; the dropped
 // lo*lo is below 2^-22 of it. TF32 pieces would need three products too, at half the rate; bf16 pieces six for the
-// same bits. The price is E, known only after the whole tensor has been seen: one more read of the tensor, which
-// leaves it in L2 for the second. A bound serves as well as the maximum (17 binades of full precision are far more than
-// needed), so dy * act'(pre) is bounded from dy alone and the gated gradients from the three tensors' own maxima.
+// the same bits. The price is E, known only after all it covers has been seen. Forward, where both operands' rows are
+// rows of the output or its columns, each row has its own and one read is enough. Backward the sums run across rows, so E
+// is the tensor's: one more read, which leaves part of it in L2 for the second. A bound serves as well as the maximum
+// (17 binades of full precision are far more than needed), so dy * act'(pre) is bounded from dy alone and the gated
+// gradients from the three tensors' own maxima.
 // Infinities and NaN do not count towards a maximum; as operands they become infinities and NaN.
 //
-// Bound by HBM: 4 B read for the maximum, 4 B read and 4 B written per value for the plane.
+// Bound by HBM: 4 B read and 4 B written per value for the plane; backward 4 B more read for the maximum.
 #include <cuda_fp16.h>
 
 #include "ffn.hpp"
@@ -30,6 +32,8 @@ __device__ __forceinline__ unsigned finite_bits(float x) {
 __device__ __forceinline__ unsigned finite_byte(unsigned byte) { return byte == 255u ? 0u : byte; }
 
 __global__ void __launch_bounds__(kThreads) k_amax(AmaxArgs a) {
+    stream_next();
+    stream_wait();
     const int s = blockIdx.y;
     const AmaxSlot t = a.slot[s];
     if ((int)blockIdx.x >= t.parts) return;
@@ -210,6 +214,10 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_cons
     __shared__ int s_exp[kMaxSlots];
     __shared__ float s_sum[8][kBlock];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    stream_next();
+    stream_wait();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.n_counters; i += kThreads) a.counters[i] = 0;
     if (warp < a.amax.slots) {
         unsigned top = 0;
         for (int i = lane; i < a.amax.slot[warp].parts; i += 32) top = max(top, __float_as_uint(a.amax.parts[warp * kAmaxParts + i]));
@@ -217,9 +225,10 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_cons
         if (lane == 0) s_exp[warp] = exponent_of(top, a.amax.slot[warp].is_ck8);
     }
     __syncthreads();
-    int ji = 0;
-    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
-        while (ji + 1 < a.jobs && unit >= a.job[ji + 1].first_unit) ji++;
+    int ji = a.jobs - 1;
+    // from the end: what the maximum's kernel read last is still in L2
+    for (int unit = a.units - 1 - (int)blockIdx.x; unit >= 0; unit -= gridDim.x) {
+        while (unit < a.job[ji].first_unit) ji--;
         const PackJob& j = a.job[ji];
         int e;
         if (j.kind == PACK_GATED) {
@@ -241,8 +250,66 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_cons
     }
 }
 
+// Planes with a scale for each row: a warp takes a row, holds it in registers between its maximum and its pieces (CHUNKS
+// times 256 values; a longer row is read again, from L2), and a block the eight rows of a group.
+template <int CHUNKS>
+__device__ __forceinline__ void pack_row(const RowJob& j, int64_t row, int lane) {
+    const bool wide = (j.cols & 7) == 0 && (reinterpret_cast<uintptr_t>(j.a) & 15) == 0;
+    const int chunks = j.col_blocks * 8;
+    const float* src = j.a + row * j.cols;
+    const bool there = row < j.rows;
+    const auto fetch = [&](int c) {
+        const int64_t left = there ? j.cols - (int64_t)c * 8 : 0;
+        return load8(src + (int64_t)c * 8, left <= 0 ? 0 : left < 8 ? (int)left : 8, wide);
+    };
+    Eight x[CHUNKS > 0 ? CHUNKS : 1];
+    unsigned top = 0;
+    if (CHUNKS > 0) {
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++) x[i] = fetch(lane + 32 * i);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = max(top, finite_bits(x[i].v[e]));
+    } else {
+#pragma unroll 4
+        for (int c = lane; c < chunks; c += 32) {
+            const Eight y = fetch(c);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = max(top, finite_bits(y.v[e]));
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int e = min(max(exponent_of(top, 0), kLeastExp), kMostExp);
+    const float scale = exp2f((float)(15 - e));
+    if (lane == 0) j.factor[row] = exp2f((float)(j.is_a ? e - 30 : e));
+    char* base = j.plane + (row >> 6) * j.col_blocks * (int64_t)(2 * kImageBytes);
+    const auto put = [&](int c, const Eight& y) { store_pieces(base + (int64_t)(c >> 3) * (int64_t)(2 * kImageBytes), 2, (int)(row & 63), c & 7, y, scale); };
+    if (CHUNKS > 0) {
+#pragma unroll
+        for (int i = 0; i < CHUNKS; i++)
+            if (lane + 32 * i < chunks) put(lane + 32 * i, x[i]);
+    } else {
+#pragma unroll 4
+        for (int c = lane; c < chunks; c += 32) put(c, fetch(c));
+    }
+}
+template <int CHUNKS>
+__global__ void __launch_bounds__(kThreads) k_rows(const __grid_constant__ RowArgs a) {
+    stream_next();
+    stream_wait();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.n_counters; i += kThreads) a.counters[i] = 0;
+    int ji = a.jobs - 1;
+    while ((int)blockIdx.x < a.job[ji].first_group) ji--;
+    const RowJob& j = a.job[ji];
+    pack_row<CHUNKS>(j, (int64_t)((int)blockIdx.x - j.first_group) * 8 + (threadIdx.x >> 5), threadIdx.x & 31);
+}
+
 // A block takes 32 columns, each of its warps every eighth block row; the eight sums meet in order.
-__global__ void __launch_bounds__(kThreads) k_colsum(const float* __restrict__ parts, int count, int64_t cols, float* __restrict__ out) {
+__global__ void __launch_bounds__(kThreads) k_colsum(const float* parts, int count, int64_t cols, float* __restrict__ out) {
+    stream_next();
+    stream_wait();
     __shared__ float part[kThreads / 32][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + lane;
@@ -261,22 +328,25 @@ __global__ void __launch_bounds__(kThreads) k_colsum(const float* __restrict__ p
     }
 }
 
+cudaError_t launch_rows(const RowArgs& a, cudaStream_t st) {
+    const int blocks = a.job[0].col_blocks;  // of 64 columns: four to a chunk of 256; all jobs have the same
+    const auto kernel = blocks <= 4 ? k_rows<1> : blocks <= 8 ? k_rows<2> : blocks <= 12 ? k_rows<3> : blocks <= 16 ? k_rows<4> : blocks <= 32 ? k_rows<8> : k_rows<0>;
+    return launch_early(kernel, dim3((unsigned)a.groups), kThreads, 0, st, 1, a);
+}
+
 cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {
     int most = 1;
     for (int s = 0; s < a.slots; s++) most = most > a.slot[s].parts ? most : a.slot[s].parts;
-    k_amax<<<dim3((unsigned)most, (unsigned)a.slots), kThreads, 0, st>>>(a);
-    return cudaPeekAtLastError();
+    return launch_early(k_amax, dim3((unsigned)most, (unsigned)a.slots), kThreads, 0, st, 1, a);
 }
 
 cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st) {
     const int most = sm_count * kPackPerSM;  // as many as run at once: each starts with the maxima
-    k_pack<<<a.units < most ? a.units : most, kThreads, 0, st>>>(a);
-    return cudaPeekAtLastError();
+    return launch_early(k_pack, dim3((unsigned)(a.units < most ? a.units : most)), kThreads, 0, st, 1, a);
 }
 
 cudaError_t launch_colsum(const float* parts, int count, int64_t cols, float* out, cudaStream_t st) {
-    k_colsum<<<(unsigned)((cols + 31) / 32), kThreads, 0, st>>>(parts, count, cols, out);
-    return cudaPeekAtLastError();
+    return launch_early(k_colsum, dim3((unsigned)((cols + 31) / 32)), kThreads, 0, st, 1, parts, count, cols, out);
 }
 
 }  // namespace slb_ffn
