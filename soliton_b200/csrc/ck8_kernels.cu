@@ -70,62 +70,67 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __re
     }
 }
 
-// Any columns, any alignment: a warp per group, a lane per column, four groups of a warp in flight.
-__global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__ x, char* __restrict__ ck, int64_t rows, int64_t cols) {
+// Any columns, any alignment: a warp per group, a lane per column, eight groups of a warp in flight.
+constexpr int kAheadAny = 8;
+struct Spot {
+    int64_t at;         // element, or -1 where the lane has none
+    int64_t group;
+};
+__device__ __forceinline__ void find_spots(Spot (&s)[kAheadAny], int64_t rows, int64_t cols) {
     const int lane = threadIdx.x & 31;
-    const int64_t groups = ck8_groups(cols), total = rows * groups;
-    const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAhead;
-    unsigned char* eb = reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols);
-    int64_t row = first / groups, g = first - row * groups, at[kAhead];
-    float v[kAhead];
-    bool ok[kAhead];
+    const int64_t groups = ck8_groups(cols), first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAheadAny;
+    int64_t row = first / groups, g = first - row * groups;
 #pragma unroll
-    for (int i = 0; i < kAhead; i++) {
-        ok[i] = first + i < total && g * kGroup + lane < cols;
-        at[i] = row * cols + g * kGroup + lane;
-        v[i] = ok[i] ? __ldcs(x + at[i]) : 0.0f;
+    for (int i = 0; i < kAheadAny; i++) {
+        s[i].group = first + i;
+        s[i].at = row < rows && g * kGroup + lane < cols ? row * cols + g * kGroup + lane : -1;
         if (++g == groups) g = 0, row++;
     }
+}
+__global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__ x, char* __restrict__ ck, int64_t rows, int64_t cols) {
+    const int lane = threadIdx.x & 31;
+    const int64_t total = rows * ck8_groups(cols);
+    unsigned char* eb = reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols);
+    Spot s[kAheadAny];
+    float v[kAheadAny];
+    find_spots(s, rows, cols);
 #pragma unroll
-    for (int i = 0; i < kAhead; i++) {
-        if (first + i >= total) break;
+    for (int i = 0; i < kAheadAny; i++) v[i] = s[i].at >= 0 ? __ldcs(x + s[i].at) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAheadAny; i++) {
+        if (s[i].group >= total) break;
         const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
-        if (ok[i]) ck[at[i]] = (char)ck8_quantise(v[i], byte);
-        if (lane == 0) eb[first + i] = (unsigned char)byte;
+        if (s[i].at >= 0) ck[s[i].at] = (char)ck8_quantise(v[i], byte);
+        if (lane == 0) eb[s[i].group] = (unsigned char)byte;
     }
 }
 
 template <bool GELU_BWD>
 __global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ ck, const float* __restrict__ dy, float* __restrict__ out, int64_t rows,
                                                        int64_t cols) {
-    const int lane = threadIdx.x & 31;
-    const int64_t groups = ck8_groups(cols), total = rows * groups;
-    const int64_t first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAhead;
     const unsigned char* eb = reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols);
-    int64_t row = first / groups, g = first - row * groups, at[kAhead];
-    float d[kAhead];
-    int q[kAhead];
-    unsigned byte[kAhead];
-    bool ok[kAhead];
+    Spot s[kAheadAny];
+    float d[kAheadAny];
+    int q[kAheadAny];
+    unsigned byte[kAheadAny];
+    find_spots(s, rows, cols);
 #pragma unroll
-    for (int i = 0; i < kAhead; i++) {
-        ok[i] = first + i < total && g * kGroup + lane < cols;
-        at[i] = row * cols + g * kGroup + lane;
-        q[i] = ok[i] ? (signed char)__ldcs(ck + at[i]) : 0;
-        byte[i] = ok[i] ? __ldg(eb + first + i) : 0u;
-        d[i] = GELU_BWD && ok[i] ? __ldcs(dy + at[i]) : 0.0f;
-        if (++g == groups) g = 0, row++;
-    }
+    for (int i = 0; i < kAheadAny; i++)
+        if (s[i].at >= 0) {
+            q[i] = (signed char)__ldg(ck + s[i].at);
+            byte[i] = __ldg(eb + s[i].group);
+            if (GELU_BWD) d[i] = __ldcs(dy + s[i].at);
+        }
 #pragma unroll
-    for (int i = 0; i < kAhead; i++)
-        if (ok[i]) __stcs(out + at[i], read_value<GELU_BWD>((float)q[i] * ck8_step(byte[i]), d[i]));
+    for (int i = 0; i < kAheadAny; i++)
+        if (s[i].at >= 0) out[s[i].at] = read_value<GELU_BWD>((float)q[i] * ck8_step(byte[i]), GELU_BWD ? d[i] : 0.0f);
 }
 
 static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 static bool wide(int64_t cols, const void* ck, const float* a, const float* b) { return cols % kGroup == 0 && aligned(ck, 4) && aligned(a, 16) && aligned(b, 16); }
 static unsigned wide_grid(int64_t rows, int64_t cols) { return (unsigned)((rows * cols / 4 + kThreads * kAhead - 1) / (kThreads * kAhead)); }
 static unsigned any_grid(int64_t rows, int64_t cols) {
-    const int64_t per_block = kThreads / 32 * kAhead;
+    const int64_t per_block = kThreads / 32 * kAheadAny;
     return (unsigned)((rows * ck8_groups(cols) + per_block - 1) / per_block);
 }
 

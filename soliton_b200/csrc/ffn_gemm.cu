@@ -452,8 +452,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) tmem_alloc<CTAS>(smem_addr(words + 1));
-    stream_next();
-    stream_wait();
+    stream_wait();  // and no stream_next(): blocks of a following product, each an SM's worth, made this one slower (231 us against 223)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     team_sync<CTAS>();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -647,17 +646,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 
 // ---------------------------------------------------------------- how a product is cut
 
-// Estimated cycles of a way of cutting: rounds of whole tiles, then the slices. A k-block takes a pair 1,750 cycles, bound by
-// what the L2 delivers, and a single block, which fetches as much for half the work, the same when most SMs run, 1,100
-// when few do; a tile's first fetches and what of its epilogue nothing covers 9,000 (6,000 single); a slice's sums are
-// written once and read once, 3,000 each (1,500).
+// Estimated cycles of a way of cutting: rounds of whole tiles, then rounds of slices. A k-block takes a pair 1,750 cycles,
+// bound by what the L2 delivers, and a single block, which fetches as much for half the work, the same when most SMs run,
+// 1,100 when few do; a tile's first fetches and what of its epilogue nothing covers 9,000 (6,000 single); a slice's sums
+// are written once and read once, 3,000 each (1,500).
 static double cut_cost(int ctas, int64_t tiles, int64_t k_blocks, int64_t slices) {
     const int64_t teams = kPlanSMs / ctas, rounds = tiles / teams, rest = tiles % teams;
     const int64_t busy = rounds > 0 ? kPlanSMs : rest * slices * ctas;
     const double block = ctas == 2 || busy > 100 ? 1750 : 1100, tile = ctas == 2 ? 9000 : 6000, slice = ctas == 2 ? 3000 : 1500;
     double t = (double)rounds * (block * (double)k_blocks + tile);
-    if (rest) t += block * (double)((k_blocks + slices - 1) / slices) + tile + (slices > 1 ? slice * (double)(1 + slices) : 0.0);
-    return t;
+    if (rest) t += (double)((rest * slices + teams - 1) / teams) * (block * (double)((k_blocks + slices - 1) / slices) + tile);
+    return slices > 1 ? t + slice * (double)(1 + slices) : t;
 }
 
 GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks) {
@@ -666,8 +665,7 @@ GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks) {
     for (int ctas = 1; ctas <= 2; ctas++) {
         const int64_t mt = (m_blocks + 2 * ctas - 1) / (2 * ctas), nt = (n_blocks + 2 * ctas - 1) / (2 * ctas), tiles = mt * nt;
         const int64_t teams = kPlanSMs / ctas, rest = tiles % teams;
-        const int64_t most = rest ? teams / rest : 1;
-        for (int64_t s = 1; s <= most && s <= k_blocks && s <= 16; s++) {
+        for (int64_t s = 1; s <= k_blocks && s <= 16 && (s == 1 || rest * s <= 3 * teams); s++) {
             const double t = cut_cost(ctas, tiles, k_blocks, s);
             if (best.ctas && t >= least) continue;
             least = t;

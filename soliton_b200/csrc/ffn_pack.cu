@@ -225,10 +225,9 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_cons
         if (lane == 0) s_exp[warp] = exponent_of(top, a.amax.slot[warp].is_ck8);
     }
     __syncthreads();
-    int ji = a.jobs - 1;
-    // from the end: what the maximum's kernel read last is still in L2
-    for (int unit = a.units - 1 - (int)blockIdx.x; unit >= 0; unit -= gridDim.x) {
-        while (unit < a.job[ji].first_unit) ji--;
+    int ji = 0;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        while (ji + 1 < a.jobs && unit >= a.job[ji + 1].first_unit) ji++;
         const PackJob& j = a.job[ji];
         int e;
         if (j.kind == PACK_GATED) {

@@ -121,14 +121,14 @@ def test_meta_takes_the_scratch_from_the_pool(lib):
 
 def test_scratch_covers_the_planes(lib):
     """Four bytes a value of the operands, whole blocks of 64; the column sums; and no more than what the sums of cut tiles
-    need: 74 accumulators of 256 x 256 at the most."""
+    need: 3 x 74 accumulators of 256 x 256 at the most."""
     def blocks(n):
         return (n + 63) // 64
 
     for m, n, k in ((1, 1, 1), (64, 64, 64), (65, 129, 193), (8192, 768, 768), (768, 8192, 100)):
         fwd = 16384 * (blocks(m) * blocks(k) + blocks(n) * blocks(k))
         bwd = fwd + 16384 * blocks(m) * blocks(n) + 4 * blocks(m) * n
-        cut = 74 * 256 * 256 * 4 + 16 * 1024
+        cut = 3 * 74 * 256 * 256 * 4 + 16 * 1024
         assert fwd <= lib.slb_linear_scratch_bytes(m, n, k, 0) <= fwd + 256 * (blocks(m) + blocks(n)) + cut
         assert bwd <= lib.slb_linear_scratch_bytes(m, n, k, 1) <= bwd + cut
         assert lib.slb_gated_scratch_bytes(m, n, k, 1) >= bwd
