@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __re
     }
 }
 
-// Any columns, any alignment: a warp per group, a lane per column, eight groups of a warp in flight.
-constexpr int kAheadAny = 8;
+// Any columns, any alignment: a warp per group, a lane per column, four groups of a warp in flight.
+constexpr int kAheadAny = 4;
 struct Spot {
     int64_t at;         // element, or -1 where the lane has none
     int64_t group;
@@ -105,6 +105,53 @@ __global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__
     }
 }
 
+// Aligned buffers, any columns from 32 up: values run on without a break even where groups do not, so a thread takes four
+// neighbours wherever they lie and follows the groups, which are numbered in the same order. One division a thread.
+template <bool GELU_BWD, class Index>
+__global__ void __launch_bounds__(kThreads) k_ck8_read_flat(const unsigned* __restrict__ q, const unsigned char* __restrict__ eb, const float* __restrict__ dy,
+                                                            float* __restrict__ out, Index total, Index cols) {
+    constexpr int kQuads = 2;
+    const Index groups = (cols + kGroup - 1) / kGroup;
+    const Index first = (Index)blockIdx.x * (kThreads * kQuads) + threadIdx.x;
+    unsigned w[kQuads], byte[kQuads][4];
+    float4 d[kQuads];
+#pragma unroll
+    for (int i = 0; i < kQuads; i++) {
+        const Index at = (first + i * kThreads) * 4;
+        if (at >= total) break;
+        w[i] = __ldcs(q + (at >> 2));  // the bytes behind the last value belong to the buffer
+        if (GELU_BWD) {
+            if (at + 4 <= total) d[i] = __ldcs(reinterpret_cast<const float4*>(dy + at));
+            else d[i] = make_float4(dy[at], at + 1 < total ? dy[at + 1] : 0.0f, at + 2 < total ? dy[at + 2] : 0.0f, 0.0f);
+        }
+        const Index row = at / cols;
+        Index col = at - row * cols, group = row * groups + (col / kGroup);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            byte[i][j] = at + j < total ? __ldg(eb + group) : 0u;
+            if (++col == cols) col = 0, group++;
+            else group += (col % kGroup) == 0;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kQuads; i++) {
+        const Index at = (first + i * kThreads) * 4;
+        if (at >= total) break;
+        float4 o;
+        o.x = read_value<GELU_BWD>((float)(signed char)w[i] * ck8_step(byte[i][0]), GELU_BWD ? d[i].x : 0.0f);
+        o.y = read_value<GELU_BWD>((float)(signed char)(w[i] >> 8) * ck8_step(byte[i][1]), GELU_BWD ? d[i].y : 0.0f);
+        o.z = read_value<GELU_BWD>((float)(signed char)(w[i] >> 16) * ck8_step(byte[i][2]), GELU_BWD ? d[i].z : 0.0f);
+        o.w = read_value<GELU_BWD>((float)(signed char)(w[i] >> 24) * ck8_step(byte[i][3]), GELU_BWD ? d[i].w : 0.0f);
+        if (at + 4 <= total) {
+            __stcs(reinterpret_cast<float4*>(out + at), o);
+        } else {
+            out[at] = o.x;
+            if (at + 1 < total) out[at + 1] = o.y;
+            if (at + 2 < total) out[at + 2] = o.z;
+        }
+    }
+}
+
 template <bool GELU_BWD>
 __global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ ck, const float* __restrict__ dy, float* __restrict__ out, int64_t rows,
                                                        int64_t cols) {
@@ -127,7 +174,8 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ 
 }
 
 static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-static bool wide(int64_t cols, const void* ck, const float* a, const float* b) { return cols % kGroup == 0 && aligned(ck, 4) && aligned(a, 16) && aligned(b, 16); }
+static bool flat(const void* ck, const float* a, const float* b) { return aligned(ck, 4) && aligned(a, 16) && aligned(b, 16); }
+static bool wide(int64_t cols, const void* ck, const float* a, const float* b) { return cols % kGroup == 0 && flat(ck, a, b); }
 static unsigned wide_grid(int64_t rows, int64_t cols) { return (unsigned)((rows * cols / 4 + kThreads * kAhead - 1) / (kThreads * kAhead)); }
 static unsigned any_grid(int64_t rows, int64_t cols) {
     const int64_t per_block = kThreads / 32 * kAheadAny;
@@ -148,7 +196,14 @@ static cudaError_t launch_read(const char* ck, const float* dy, float* out, int6
         k_ck8_read_wide<GELU_BWD><<<wide_grid(rows, cols), kThreads, 0, st>>>(reinterpret_cast<const unsigned*>(ck),
                                                                             reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols),
                                                                             reinterpret_cast<const float4*>(dy), reinterpret_cast<float4*>(out), rows * cols / 4);
-    else
+    else if (cols >= kGroup && flat(ck, dy, out)) {
+        const int64_t total = rows * cols;
+        const unsigned grid = (unsigned)(((total + 3) / 4 + 2 * kThreads - 1) / (2 * kThreads));
+        const unsigned* q = reinterpret_cast<const unsigned*>(ck);
+        const unsigned char* eb = reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols);
+        if (total < (int64_t(1) << 31)) k_ck8_read_flat<GELU_BWD, unsigned><<<grid, kThreads, 0, st>>>(q, eb, dy, out, (unsigned)total, (unsigned)cols);
+        else k_ck8_read_flat<GELU_BWD, int64_t><<<grid, kThreads, 0, st>>>(q, eb, dy, out, total, cols);
+    } else
         k_ck8_read<GELU_BWD><<<any_grid(rows, cols), kThreads, 0, st>>>(ck, dy, out, rows, cols);
     return cudaPeekAtLastError();
 }
