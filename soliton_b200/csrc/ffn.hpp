@@ -31,11 +31,13 @@ struct AmaxSlot {
     int64_t n;
     int is_ck8;
     int parts;                      // partial maxima, at most kAmaxParts
+    int sampled;                    // only a sixteenth is read: 4 KiB in every 64
 };
 struct AmaxArgs {
     AmaxSlot slot[kMaxSlots];
     int slots;
     float* parts;                   // kMaxSlots x kAmaxParts
+    unsigned* tops;                 // zeroed here, for the planes of a sampled maximum
 };
 
 enum PackKind : int {
@@ -65,6 +67,9 @@ struct PackArgs {
     PackJob job[kMaxJobs];
     int jobs, units;
     AmaxArgs amax;
+    int planes;                     // with sampled maxima: all planes of the call have jobs
+    int sampled;
+    int* guess;                     // sampled: the exponents of the first pass
     int* exps;                      // out: values of plane i were multiplied by 2^(15 - exps[i])
     int* counters;                  // to be zeroed for the products that follow
     int n_counters;
@@ -132,8 +137,10 @@ GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks);
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t st);
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
 cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st);
-// out[j] = the sum over `parts` of the block rows' column sums, in order
-cudaError_t launch_colsum(const float* parts, int count, int64_t cols, float* out, cudaStream_t st);
+// After a pack with sampled maxima: does planes again whose values went beyond what their exponent allows.
+cudaError_t launch_repack(const PackArgs& a, int sm_count, cudaStream_t st);
+// out[j] = the sum over `parts` of the block rows' column sums, in order; the same for a second matrix where given
+cudaError_t launch_colsum(const float* parts, float* out, const float* parts2, float* out2, int count, int64_t cols, cudaStream_t st);
 // a_mn, b_mn: the operand's blocks hold K along their rows. pieces_b: 1 when B is a checkpoint's plane.
 cudaError_t launch_gemm(const GemmArgs& g, bool a_mn, bool b_mn, int pieces_b, Epilogue epi, int sm_count, cudaStream_t st);
 

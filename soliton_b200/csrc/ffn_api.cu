@@ -40,7 +40,8 @@ struct Carver {
     }
 };
 struct Scratch {
-    int* exps;
+    int *exps, *guess;
+    unsigned* tops;
     float *parts, *colsum, *colsum2;
     float *row_factor, *col_factor, *col_factor2;
     char *y, *x, *w;        // planes: the gradient of the pre-activations, the input, the weights
@@ -62,6 +63,8 @@ size_t carve(Scratch& s, void* base, int64_t m, int64_t n, int64_t k, int weight
         const int dw_counters = dw.counters > half.counters ? dw.counters : half.counters;
         s.y = c.take((size_t)(weights * mb * nb) * block);
         s.exps = reinterpret_cast<int*>(c.take(kMaxPlanes * sizeof(int)));
+        s.guess = reinterpret_cast<int*>(c.take(kMaxPlanes * sizeof(int)));
+        s.tops = reinterpret_cast<unsigned*>(c.take(kMaxPlanes * sizeof(unsigned)));
         s.parts = reinterpret_cast<float*>(c.take(kMaxSlots * kAmaxParts * sizeof(float)));
         s.colsum = reinterpret_cast<float*>(c.take((size_t)(mb * n) * sizeof(float)));
         s.colsum2 = weights == 2 ? reinterpret_cast<float*>(c.take((size_t)(mb * n) * sizeof(float))) : nullptr;
@@ -134,7 +137,9 @@ int refuse(int code) {
 
 struct Planner {
     PackArgs p{};
-    explicit Planner(const Scratch& s) { p.amax.parts = s.parts, p.exps = s.exps, p.counters = s.counters, p.n_counters = s.n_counters; }
+    explicit Planner(const Scratch& s) {
+        p.amax.parts = s.parts, p.amax.tops = s.tops, p.guess = s.guess, p.exps = s.exps, p.counters = s.counters, p.n_counters = s.n_counters;
+    }
     int slot(const float* x, const void* ck, int64_t rows, int64_t cols) {
         AmaxSlot& t = p.amax.slot[p.amax.slots];
         t.is_ck8 = x == nullptr;
@@ -142,6 +147,7 @@ struct Planner {
         t.n = x ? rows * cols : rows * ck8_groups(cols);
         const int64_t want = (t.n * (x ? 4 : 1) + 16383) / 16384;
         t.parts = (int)(want < 1 ? 1 : want < kAmaxParts ? want : kAmaxParts);
+        if (x) bytes_ += 4 * t.n;
         return p.amax.slots++;
     }
     PackJob& job(int kind, int64_t rows, int64_t cols, char* plane, int plane_id, int pieces) {
@@ -151,6 +157,7 @@ struct Planner {
         j.plane = plane, j.plane_id = plane_id, j.pieces = pieces;
         j.first_unit = p.units;
         p.units += j.row_blocks * j.col_blocks;
+        p.planes |= 1 << plane_id;
         return j;
     }
     // the matrix itself, or its checkpoint
@@ -160,9 +167,20 @@ struct Planner {
         return j;
     }
     void launch(Op& op) {
+        // Tensors that a second read would find in L2 are read whole; of more, those of 16 MiB up are sampled.
+        for (int s = 0; s < p.amax.slots && bytes_ > kReadTwice; s++) {
+            AmaxSlot& t = p.amax.slot[s];
+            t.sampled = !t.is_ck8 && t.n >= (int64_t(1) << 22);
+            p.sampled |= t.sampled;
+        }
         op.launched(launch_amax(p.amax, op.sms(), 0));
         op.launched(launch_pack(p, op.sms(), 0));
+        if (p.sampled) op.launched(launch_repack(p, op.sms(), 0));
     }
+
+private:
+    static constexpr int64_t kReadTwice = int64_t(100) << 20;
+    int64_t bytes_ = 0;
 };
 
 // Planes of a forward pass.
@@ -285,7 +303,7 @@ int run_linear_bwd(const float* dy, const float* x, const void* x8, const float*
         p.matrix(w, nullptr, n, k, s.w, PLANE_W, 1 << i);
     }
     p.launch(op);
-    if (db) op.launched(launch_colsum(s.colsum, (int)blocks_of(m), n, db, 0));
+    if (db) op.launched(launch_colsum(s.colsum, db, nullptr, nullptr, (int)blocks_of(m), n, 0));
     gradients(op, s, x8 != nullptr, dx, dw, nullptr, m, n, k, 1);
     return op.done();
 }
@@ -322,8 +340,7 @@ int run_gated_bwd(const float* dh, const float* x, const void* x8, const float* 
         p.matrix(wu, nullptr, f, k, s.w + fb * kb * (int64_t)(2 * kImageBytes), PLANE_W, 3 << i);
     }
     p.launch(op);
-    if (dbg) op.launched(launch_colsum(s.colsum, (int)blocks_of(m), f, dbg, 0));
-    if (dbu) op.launched(launch_colsum(s.colsum2, (int)blocks_of(m), f, dbu, 0));
+    if (dbg || dbu) op.launched(launch_colsum(s.colsum, dbg, s.colsum2, dbu, (int)blocks_of(m), f, 0));
     gradients(op, s, x8 != nullptr, dx, dwg, dwu, m, f, k, 2);
     return op.done();
 }

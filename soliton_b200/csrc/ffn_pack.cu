@@ -10,6 +10,12 @@
 // is the tensor's: one more read, which leaves part of it in L2 for the second. A bound serves as well as the maximum
 // (17 binades of full precision are far more than needed), so dy * act'(pre) is bounded from dy alone and the gated
 // gradients from the three tensors' own maxima.
+//
+// Large tensors do not stay in L2, and there the second read costs what the first did (38 of 352 us for the gated block's
+// gradients at 8192 x 2048 x 768). Their maxima are sampled, a sixteenth of the tensor, and E is taken kMargin higher: a
+// value may then exceed the sample's largest by 2^kMargin, and full precision still reaches
+// 2^(17 - kMargin) below. The pass that cuts the values keeps their true maximum, and a last pass, which otherwise ends at
+// once, does a plane again from the true maximum if it did overflow.
 // Infinities and NaN do not count towards a maximum; as operands they become infinities and NaN.
 //
 // Bound by HBM: 4 B read and 4 B written per value for the plane; backward 4 B more read for the maximum.
@@ -20,7 +26,9 @@
 namespace slb_ffn {
 
 constexpr int kThreads = 256;
-constexpr int kPackPerSM = 3;       // blocks of k_pack on one SM: 80 registers a thread hold two rows of three tensors
+// Blocks of k_pack on one SM: two rows of three tensors take 80 registers a thread, of two 64.
+template <bool GATED>
+constexpr int kPackPerSM = GATED ? 3 : 4;
 
 // ---------------------------------------------------------------- maxima
 
@@ -39,9 +47,18 @@ __global__ void __launch_bounds__(kThreads) k_amax(AmaxArgs a) {
     if ((int)blockIdx.x >= t.parts) return;
     unsigned top = 0;
     const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, step = (int64_t)t.parts * kThreads;
+    if (a.tops && blockIdx.x == 0 && s == 0 && threadIdx.x < kMaxPlanes) a.tops[threadIdx.x] = 0;
     if (t.is_ck8) {
         const unsigned char* p = static_cast<const unsigned char*>(t.p);
         for (int64_t i = at; i < t.n; i += step) top = max(top, finite_byte(p[i]));
+    } else if (t.sampled) {  // a 16-byte word a thread of 4 KiB in every 64; only where a tensor has many of those
+        const float4* w = reinterpret_cast<const float4*>((reinterpret_cast<uintptr_t>(t.p) + 15) & ~(uintptr_t)15);
+        const int64_t strips = (t.n - 4) / 16384;
+#pragma unroll 4
+        for (int64_t i = blockIdx.x; i < strips; i += t.parts) {
+            const float4 v = __ldg(w + i * 4096 + threadIdx.x);
+            top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+        }
     } else {
         const float* p = static_cast<const float*>(t.p);
         // up to three values ahead of the first 16-byte boundary, then 128-bit words, then the rest
@@ -80,6 +97,7 @@ __device__ __forceinline__ int exponent_of(unsigned top, int is_ck8) {
     if (is_ck8) return (int)top - 127 + 7;
     return (int)(top >> 23) - 126;
 }
+constexpr int kMargin = 6;
 constexpr int kLeastExp = -110, kMostExp = 128;  // so that 2^(15 - E) and its reciprocal are normal floats
 
 // ---------------------------------------------------------------- planes
@@ -174,14 +192,16 @@ __device__ __forceinline__ Eight load8_held(const PackJob& j, const float* p, co
 }
 
 // One block of 64 x 64: a thread takes eight columns of two rows, all of whose loads are issued before the first is used.
-template <int KIND>
-__device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scale, float (&s_sum)[8][kBlock]) {
+// TOP: the largest finite magnitude is wanted as well. SUM: column sums may be.
+template <int KIND, bool TOP, bool SUM>
+__device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scale, float (&s_sum)[8][kBlock], unsigned* top) {
     const int chunk = threadIdx.x & 7, row_in = threadIdx.x >> 3;
     const int u = unit - j.first_unit, rb = u / j.col_blocks, cb = u - rb * j.col_blocks;
     const int64_t col = (int64_t)cb * kBlock + chunk * 8;
     const int have = col >= j.cols ? 0 : j.cols - col < 8 ? (int)(j.cols - col) : 8;
     char* block = j.plane + ((int64_t)rb * j.row_stride + cb) * (int64_t)(j.pieces * kImageBytes);
     Eight x[2], y[2], z[2];
+    unsigned most = 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int64_t row = (int64_t)rb * kBlock + row_in + 32 * h;
@@ -202,15 +222,34 @@ __device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scal
                 y[h].v[i] = d * act_of(j.act, gate);
             }
         }
+        if (TOP && KIND != PACK_CK8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = max(most, KIND == PACK_GATED ? max(finite_bits(x[h].v[i]), finite_bits(y[h].v[i])) : finite_bits(x[h].v[i]));
+        }
         store_pieces(block, KIND == PACK_CK8 ? 1 : 2, r, chunk, x[h], scale);
         if (KIND == PACK_GATED) store_pieces(block + (int64_t)j.second * (int64_t)(2 * kImageBytes), 2, r, chunk, y[h], scale);
     }
-    if (KIND != PACK_CK8 && j.colsum) block_colsum(x, s_sum, j.colsum + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
-    if (KIND == PACK_GATED && j.colsum2) block_colsum(y, s_sum, j.colsum2 + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+    if (TOP && KIND != PACK_CK8) {
+        most = __reduce_max_sync(0xffffffffu, most);
+        if ((threadIdx.x & 31) == 0 && most > *reinterpret_cast<volatile unsigned*>(top)) atomicMax(top, most);
+    }
+    if (SUM && KIND != PACK_CK8 && j.colsum) block_colsum(x, s_sum, j.colsum + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
+    if (SUM && KIND == PACK_GATED && j.colsum2) block_colsum(y, s_sum, j.colsum2 + (int64_t)rb * j.cols, (int64_t)cb * kBlock, j.cols);
 }
 
-// Blocks of threads take blocks of 64 x 64 round robin over all jobs.
-__global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_constant__ PackArgs a) {
+template <bool TOP, bool SUM, bool GATED>
+__device__ __forceinline__ void pack_any(const PackJob& j, int unit, int e, float (&s_sum)[8][kBlock], unsigned* tops) {
+    const float scale = exp2f((float)(15 - e));
+    unsigned* top = tops + j.plane_id;
+    if (j.kind == PACK_FP32) pack_unit<PACK_FP32, TOP, SUM>(j, unit, scale, s_sum, top);
+    else if (j.kind == PACK_CK8) pack_unit<PACK_CK8, TOP, SUM>(j, unit, scale, s_sum, top);
+    else if (!GATED || j.kind == PACK_ACT) pack_unit<PACK_ACT, TOP, SUM>(j, unit, scale, s_sum, top);
+    else pack_unit<PACK_GATED, TOP, SUM>(j, unit, scale, s_sum, top);
+}
+
+// Blocks of threads take blocks of 64 x 64 round robin over all jobs. SAMPLED: the maxima are. GATED: a job is.
+template <bool SAMPLED, bool GATED>
+__global__ void __launch_bounds__(kThreads, kPackPerSM<GATED>) k_pack(const __grid_constant__ PackArgs a) {
     __shared__ int s_exp[kMaxSlots];
     __shared__ float s_sum[8][kBlock];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -230,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_cons
         while (ji + 1 < a.jobs && unit >= a.job[ji + 1].first_unit) ji++;
         const PackJob& j = a.job[ji];
         int e;
-        if (j.kind == PACK_GATED) {
+        if (GATED && j.kind == PACK_GATED) {
             e = s_exp[0] + max(s_exp[1] + (j.act != ACT_NONE), s_exp[2]);  // |act'| < 2, |act(g)| <= |g|
         } else if (j.kind == PACK_ACT) {
             e = s_exp[0] + 1;
@@ -239,15 +278,39 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM) k_pack(const __grid_cons
             for (int s = 0; s < a.amax.slots; s++)
                 if (j.slots >> s & 1) e = max(e, s_exp[s]);
         }
+        if (SAMPLED && j.kind != PACK_CK8) e += kMargin;
         e = min(max(e, kLeastExp), kMostExp);
-        if (unit == j.first_unit && threadIdx.x == 0) a.exps[j.plane_id] = e;
-        const float scale = exp2f((float)(15 - e));
-        if (j.kind == PACK_FP32) pack_unit<PACK_FP32>(j, unit, scale, s_sum);
-        else if (j.kind == PACK_CK8) pack_unit<PACK_CK8>(j, unit, scale, s_sum);
-        else if (j.kind == PACK_ACT) pack_unit<PACK_ACT>(j, unit, scale, s_sum);
-        else pack_unit<PACK_GATED>(j, unit, scale, s_sum);
+        if (unit == j.first_unit && threadIdx.x == 0) (SAMPLED ? a.guess : a.exps)[j.plane_id] = e;
+        pack_any<SAMPLED, true, GATED>(j, unit, e, s_sum, a.amax.tops);
     }
 }
+
+// The planes whose largest value did not fit below 2^e. (A checkpoint's exponents are never sampled, so its plane, which
+// keeps no maximum, always fits.)
+template <bool GATED>
+__global__ void __launch_bounds__(kThreads, kPackPerSM<GATED>) k_repack(const __grid_constant__ PackArgs a) {
+    __shared__ float s_sum[8][kBlock];
+    stream_next();
+    stream_wait();
+    int e[kMaxPlanes];
+    bool again[kMaxPlanes], any = false;
+    for (int p = 0; p < kMaxPlanes; p++) {
+        const int got = a.planes >> p & 1 ? a.guess[p] : 0, need = min(max(exponent_of(a.amax.tops[p], 0), kLeastExp), kMostExp);
+        again[p] = (a.planes >> p & 1) && need > got;
+        e[p] = again[p] ? need : got;
+        any |= again[p];
+        if (blockIdx.x == 0 && threadIdx.x == 0 && (a.planes >> p & 1)) a.exps[p] = e[p];
+    }
+    if (!any) return;
+    int ji = 0;
+    for (int unit = blockIdx.x; unit < a.units; unit += gridDim.x) {
+        while (ji + 1 < a.jobs && unit >= a.job[ji + 1].first_unit) ji++;
+        const PackJob& j = a.job[ji];
+        const int p = j.plane_id;
+        if (p == 0 ? again[0] : p == 1 ? again[1] : again[2]) pack_any<false, false, GATED>(j, unit, p == 0 ? e[0] : p == 1 ? e[1] : e[2], s_sum, a.amax.tops);
+    }
+}
+static_assert(kMaxPlanes == 3, "three planes by name above");
 
 // Planes with a scale for each row: a warp takes a row, holds it in registers between its maximum and its pieces (CHUNKS
 // times 256 values; a longer row is read again, from L2), and a block the eight rows of a group.
@@ -306,12 +369,13 @@ __global__ void __launch_bounds__(kThreads) k_rows(const __grid_constant__ RowAr
 }
 
 // A block takes 32 columns, each of its warps every eighth block row; the eight sums meet in order.
-__global__ void __launch_bounds__(kThreads) k_colsum(const float* parts, int count, int64_t cols, float* __restrict__ out) {
-    stream_next();
-    stream_wait();
+__global__ void __launch_bounds__(kThreads) k_colsum(const float* parts, float* out, const float* parts2, float* out2, int count, int64_t cols) {
     __shared__ float part[kThreads / 32][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+    if (blockIdx.y == 1) parts = parts2, out = out2;
+    stream_next();
+    stream_wait();
     float sum = 0;
     if (j < cols) {
 #pragma unroll 8
@@ -339,13 +403,23 @@ cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {
     return launch_early(k_amax, dim3((unsigned)most, (unsigned)a.slots), kThreads, 0, st, 1, a);
 }
 
+static bool gated(const PackArgs& a) { return a.job[0].kind == PACK_GATED; }  // it comes first
+static dim3 pack_grid(const PackArgs& a, int sm_count) {
+    const int most = sm_count * (gated(a) ? kPackPerSM<true> : kPackPerSM<false>);  // as many as run at once: each starts with the maxima
+    return dim3((unsigned)(a.units < most ? a.units : most));
+}
 cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st) {
-    const int most = sm_count * kPackPerSM;  // as many as run at once: each starts with the maxima
-    return launch_early(k_pack, dim3((unsigned)(a.units < most ? a.units : most)), kThreads, 0, st, 1, a);
+    const auto kernel = gated(a) ? (a.sampled ? k_pack<true, true> : k_pack<false, true>) : (a.sampled ? k_pack<true, false> : k_pack<false, false>);
+    return launch_early(kernel, pack_grid(a, sm_count), kThreads, 0, st, 1, a);
+}
+cudaError_t launch_repack(const PackArgs& a, int sm_count, cudaStream_t st) {
+    return launch_early(gated(a) ? k_repack<true> : k_repack<false>, pack_grid(a, sm_count), kThreads, 0, st, 1, a);
 }
 
-cudaError_t launch_colsum(const float* parts, int count, int64_t cols, float* out, cudaStream_t st) {
-    return launch_early(k_colsum, dim3((unsigned)((cols + 31) / 32)), kThreads, 0, st, 1, parts, count, cols, out);
+cudaError_t launch_colsum(const float* parts, float* out, const float* parts2, float* out2, int count, int64_t cols, cudaStream_t st) {
+    const bool first = out != nullptr, both = first && out2;
+    return launch_early(k_colsum, dim3((unsigned)((cols + 31) / 32), both ? 2u : 1u), kThreads, 0, st, 1, first ? parts : parts2, first ? out : out2, parts2, out2, count,
+                        cols);
 }
 
 }  // namespace slb_ffn

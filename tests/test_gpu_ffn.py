@@ -174,3 +174,49 @@ def test_gated_bwd(m, n, k, kind, held8):
                 close(o.get(*f.shape), *wants[i])
             else:
                 np.testing.assert_array_equal(o.get(*f.shape), f)
+
+
+@pytest.mark.parametrize("outlier", [None, 3e4, 1e30])
+def test_sampled_maxima(outlier):
+    """Gradients of tensors large enough to be sampled for their scale, also where the largest value is one that the sample
+    (4 KiB in every 64) does not see."""
+    m, n, k = 6000, 4500, 72
+    rng = np.random.default_rng(17)
+    x, w, dy = normal(rng, m, k), normal(rng, n, k, std=0.1), normal(rng, m, n, std=1e-3)
+    if outlier is not None:
+        dy.reshape(-1)[16384 * 40 + 8000] = outlier
+    bx, bw, bdy = DevBuf(x), DevBuf(w), DevBuf(dy)
+    a, b, c = Out(m * k), Out(n * k), Out(n)
+    before = counter("launches")
+    assert lib.slb_linear_bwd(CUDA, bdy.ptr, bx.ptr, None, bw.ptr, None, None, a.ptr, b.ptr, c.ptr, m, n, k, 0) == 0
+    check_ok()
+    assert counter("launches") - before == 6  # maxima, planes, planes again, column sums, two products
+    dx, dw, db, d = ops.linear_bwd(dy, x, w)
+    ad, ax, aw = np.abs(d), np.abs(x).astype(np.float64), np.abs(w).astype(np.float64)
+    # with one scale for the whole tensor, values below 2^-11 of the largest have an absolute error of 2^-34 of it
+    floor = np.full(ad.shape, 2.0 ** -34 * ad.max())
+    close(a.get(m, k), dx, product_bound(n, ad @ aw) + floor @ aw, "dx")
+    close(b.get(n, k), dw, product_bound(m, ad.T @ ax) + floor.T @ ax, "dw")
+    close(c.get(n), db, T * (m + 8) * ad.sum(0), "db")
+
+
+def test_gated_gradients_with_sampled_maxima():
+    m, n, k = 3600, 2500, 136
+    rng = np.random.default_rng(18)
+    x, wg, wu = normal(rng, m, k), normal(rng, n, k, std=0.1), normal(rng, n, k, std=0.1)
+    g, u, dh = normal(rng, m, n), normal(rng, m, n), normal(rng, m, n, std=1e-3)
+    u.reshape(-1)[16384 * 30 + 9001] = 5e5
+    bufs = [DevBuf(t) for t in (dh, x, wg, wu, g, u)]
+    outs = [Out(m * k), Out(n * k), Out(n * k), Out(n), Out(n)]
+    bdh, bx, bwg, bwu, bg, bu = (b.ptr for b in bufs)
+    assert lib.slb_gated_bwd(CUDA, bdh, bx, None, bwg, bwu, bg, bu, None, None, *[o.ptr for o in outs], m, n, k, ops.ACTS["silu"]) == 0
+    check_ok()
+    dx, dwg, dwu, dbg, dbu, dg, du = ops.gated_bwd(dh, x, wg, wu, g, u, "silu")
+    ax, awg, awu = (np.abs(t).astype(np.float64) for t in (x, wg, wu))
+    top = max(np.abs(dg).max(), np.abs(du).max())
+    eg = 16 * T * np.abs(dh) * np.abs(u) * (1 + np.abs(g)) + 2.0 ** -34 * top
+    eu = 14 * T * np.abs(dh) * np.abs(g) + 2.0 ** -34 * top
+    ag, au = np.abs(dg), np.abs(du)
+    close(outs[0].get(m, k), dx, product_bound(2 * n, ag @ awg + au @ awu) + eg @ awg + eu @ awu, "dx")
+    close(outs[1].get(n, k), dwg, product_bound(m, ag.T @ ax) + eg.T @ ax, "dwg")
+    close(outs[2].get(n, k), dwu, product_bound(m, au.T @ ax) + eu.T @ ax, "dwu")
