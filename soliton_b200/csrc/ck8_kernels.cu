@@ -62,10 +62,10 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __re
         if (at >= quads) break;
         const float step = ck8_step(byte[i]);
         float4 o;
-        o.x = read_value<GELU_BWD>((float)(signed char)w[i] * step, GELU_BWD ? d[i].x : 0.0f);
-        o.y = read_value<GELU_BWD>((float)(signed char)(w[i] >> 8) * step, GELU_BWD ? d[i].y : 0.0f);
-        o.z = read_value<GELU_BWD>((float)(signed char)(w[i] >> 16) * step, GELU_BWD ? d[i].z : 0.0f);
-        o.w = read_value<GELU_BWD>((float)(signed char)(w[i] >> 24) * step, GELU_BWD ? d[i].w : 0.0f);
+        o.x = read_value<GELU_BWD>(ck8_integer<0>(w[i]) * step, GELU_BWD ? d[i].x : 0.0f);
+        o.y = read_value<GELU_BWD>(ck8_integer<1>(w[i]) * step, GELU_BWD ? d[i].y : 0.0f);
+        o.z = read_value<GELU_BWD>(ck8_integer<2>(w[i]) * step, GELU_BWD ? d[i].z : 0.0f);
+        o.w = read_value<GELU_BWD>(ck8_integer<3>(w[i]) * step, GELU_BWD ? d[i].w : 0.0f);
         __stcs(out + at, o);
     }
 }
@@ -138,10 +138,10 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_flat(const unsigned* __re
         const Index at = (first + i * kThreads) * 4;
         if (at >= total) break;
         float4 o;
-        o.x = read_value<GELU_BWD>((float)(signed char)w[i] * ck8_step(byte[i][0]), GELU_BWD ? d[i].x : 0.0f);
-        o.y = read_value<GELU_BWD>((float)(signed char)(w[i] >> 8) * ck8_step(byte[i][1]), GELU_BWD ? d[i].y : 0.0f);
-        o.z = read_value<GELU_BWD>((float)(signed char)(w[i] >> 16) * ck8_step(byte[i][2]), GELU_BWD ? d[i].z : 0.0f);
-        o.w = read_value<GELU_BWD>((float)(signed char)(w[i] >> 24) * ck8_step(byte[i][3]), GELU_BWD ? d[i].w : 0.0f);
+        o.x = read_value<GELU_BWD>(ck8_integer<0>(w[i]) * ck8_step(byte[i][0]), GELU_BWD ? d[i].x : 0.0f);
+        o.y = read_value<GELU_BWD>(ck8_integer<1>(w[i]) * ck8_step(byte[i][1]), GELU_BWD ? d[i].y : 0.0f);
+        o.z = read_value<GELU_BWD>(ck8_integer<2>(w[i]) * ck8_step(byte[i][2]), GELU_BWD ? d[i].z : 0.0f);
+        o.w = read_value<GELU_BWD>(ck8_integer<3>(w[i]) * ck8_step(byte[i][3]), GELU_BWD ? d[i].w : 0.0f);
         if (at + 4 <= total) {
             __stcs(reinterpret_cast<float4*>(out + at), o);
         } else {

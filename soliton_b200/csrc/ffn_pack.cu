@@ -125,11 +125,8 @@ __device__ __forceinline__ Eight load8_ck(const void* ck, int64_t rows, int64_t 
     Eight r;
     if (wide && have == 8) {
         const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            r.v[i] = (float)(signed char)(w.x >> (8 * i)) * step;
-            r.v[4 + i] = (float)(signed char)(w.y >> (8 * i)) * step;
-        }
+        r.v[0] = ck8_integer<0>(w.x) * step, r.v[1] = ck8_integer<1>(w.x) * step, r.v[2] = ck8_integer<2>(w.x) * step, r.v[3] = ck8_integer<3>(w.x) * step;
+        r.v[4] = ck8_integer<0>(w.y) * step, r.v[5] = ck8_integer<1>(w.y) * step, r.v[6] = ck8_integer<2>(w.y) * step, r.v[7] = ck8_integer<3>(w.y) * step;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) r.v[i] = i < have ? (float)__ldg(q + i) * step : 0.0f;
