@@ -104,6 +104,7 @@ enum Epilogue : int { EPI_STORE = 0, EPI_LINEAR = 1, EPI_GATED = 2 };
 struct GemmArgs {
     Operand a, b;
     int k_blocks;
+    int64_t k_len;                  // terms that exist (for the gated block's two products side by side: blocks' worth)
     int m_tiles, n_tiles;           // set by launch_gemm
     const int* exps;                // EPI_STORE
     const float *row_factor, *col_factor, *col_factor2;  // otherwise: of the rows of A and of B (EPI_GATED: of its two weights)

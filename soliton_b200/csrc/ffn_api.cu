@@ -223,7 +223,7 @@ int run_linear(const float* x, const float* w, const float* bias, const float* r
     GemmArgs g = product(op, s);
     const int64_t kb = blocks_of(k);
     g.a = k_major(s.x, blocks_of(m), kb, PLANE_X), g.b = k_major(s.w, blocks_of(n), kb, PLANE_W);
-    g.k_blocks = (int)kb, g.rows = m, g.cols = n, g.act = act;
+    g.k_blocks = (int)kb, g.k_len = k, g.rows = m, g.cols = n, g.act = act;
     g.out = y, g.bias = bias, g.residual = residual, g.save = pre, g.save8 = static_cast<char*>(pre8);
     op.launched(launch_gemm(g, false, false, 2, EPI_LINEAR, op.sms(), 0));
     return op.done();
@@ -245,7 +245,7 @@ int run_gated(const float* x, const float* wg, const float* wu, const float* bg,
     op.launched(launch_rows(p.r, 0));
     GemmArgs g = product(op, s);
     g.a = k_major(s.x, blocks_of(m), kb, PLANE_X), g.b = k_major(s.w, 2 * fb, kb, PLANE_W);
-    g.k_blocks = (int)kb, g.rows = m, g.cols = f, g.act = act, g.gate_blocks = (int)fb;
+    g.k_blocks = (int)kb, g.k_len = k, g.rows = m, g.cols = f, g.act = act, g.gate_blocks = (int)fb;
     g.out = h, g.bias = bg, g.bias2 = bu, g.save = gate, g.save2 = up, g.save8 = static_cast<char*>(gate8), g.save8_2 = static_cast<char*>(up8);
     op.launched(launch_gemm(g, false, false, 2, EPI_GATED, op.sms(), 0));
     return op.done();
@@ -258,7 +258,7 @@ void gradients(Op& op, const Scratch& s, bool x_ck8, float* dx, float* dw, float
     if (dx) {
         GemmArgs g = product(op, s);
         g.a = k_major(s.y, mb, width, PLANE_Y), g.b = mn_major(s.w, kb, kb, PLANE_W);
-        g.k_blocks = (int)width, g.rows = m, g.cols = k, g.out = dx;
+        g.k_blocks = (int)width, g.k_len = halves == 2 ? width * kBlock : n, g.rows = m, g.cols = k, g.out = dx;
         op.launched(launch_gemm(g, false, true, 2, EPI_STORE, op.sms(), 0));
     }
     if (dw || dw2) {
@@ -268,7 +268,7 @@ void gradients(Op& op, const Scratch& s, bool x_ck8, float* dx, float* dw, float
         GemmArgs g = product(op, s);
         g.counters += gemm_plan(mb, kb, width).counters;  // behind dx's
         g.a = mn_major(y, both ? width : nb, width, PLANE_Y), g.b = mn_major(s.x, kb, kb, PLANE_X);
-        g.k_blocks = (int)mb, g.rows = n, g.cols = k, g.out = dw ? dw : dw2;
+        g.k_blocks = (int)mb, g.k_len = m, g.rows = n, g.cols = k, g.out = dw ? dw : dw2;
         if (both) g.split = nb * kBlock, g.out2 = dw2;
         op.launched(launch_gemm(g, true, true, x_ck8 ? 1 : 2, EPI_STORE, op.sms(), 0));
     }

@@ -6,8 +6,8 @@
 // x 16 each into an accumulator in tensor memory. K-major and MN-major operands read the same image through different
 // descriptors.
 //
-// The tensor cores round every accumulation towards zero, so a long sum drifts by about half an ulp per step. Sums are
-// therefore cut into segments of 256 to 384 along K: the accumulator has two buffers, the warps of the epilogue add a finished
+// The tensor cores round every accumulation towards zero, so a long sum drifts, by 0.14 ulps a step on the average. That
+// much is given back (segment_gain), and sums are cut into segments of 256 to 384 along K: the accumulator has two buffers, the warps of the epilogue add a finished
 // segment to fp32 registers (to nearest) while the next one runs in the other buffer. The same double buffer lets a
 // tile's epilogue run under the next tile's products: blocks are persistent, one per SM.
 //
@@ -138,8 +138,8 @@ __device__ __forceinline__ void give_up(const GemmArgs& g, volatile int* stop) {
     *stop = 1;
     if (g.status) *reinterpret_cast<volatile int*>(g.status) = slb::ST_TIMEOUT_PRODUCT;
 }
-// Adds 16 columns of the warp's 32 rows of tensor memory to `sum`.
-__device__ __forceinline__ void tmem_add16(unsigned addr, float* sum) {
+// Adds 16 columns of the warp's 32 rows of tensor memory, times `gain`, to `sum`.
+__device__ __forceinline__ void tmem_add16(unsigned addr, float gain, float* sum) {
     unsigned r[16];
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
@@ -147,7 +147,7 @@ __device__ __forceinline__ void tmem_add16(unsigned addr, float* sum) {
                  : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; i++) sum[i] += __uint_as_float(r[i]);
+    for (int i = 0; i < 16; i++) sum[i] = fmaf(__uint_as_float(r[i]), gain, sum[i]);
 }
 
 // Shared-memory descriptors of blocks (128-byte swizzle; groups of eight 128-byte rows lie 1 KiB apart for each piece).
@@ -180,6 +180,17 @@ __device__ __forceinline__ constexpr unsigned column_of(int half, int c) {
 }
 
 // ---------------------------------------------------------------- epilogue
+
+// What a segment of `terms` along K lost on the average to rounding towards zero, given back. An accumulation loses half
+// an ulp of the sum so far, 0.36 * 2^-23 of it over all mantissas, and the sum so far is half the final one on the
+// average: 0.18 * 2^-23 of the segment a step. Measured, 1024 x 1024 results over 768 to 4096 terms, least squares against
+// 64 bits: 0.14 for normal factors, 0.15 with a mean of half their deviation, 0.30 where all products are positive, 0.07
+// where 95 % of one factor are zeros. With 0.14 the error at 1024 normal terms halves, 1.31e-6 to 0.7e-6 (fp32 sums: 0.57e-6);
+// sums that would have been exact come out that much too large instead of those too small.
+template <int PB>
+__device__ __forceinline__ float segment_gain(int64_t terms) {
+    return 1.0f + 0.14f * 1.1920929e-7f * (float)((1 + PB) * (int)((terms + 15) >> 4));
+}
 
 struct Piece {          // rows x 32 columns of the output
     int64_t row0, col0;
@@ -595,13 +606,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
             const int k_blocks = at.k1 - at.k0;
             for (int k0 = 0; k0 < k_blocks; k0 = segment_end(k0, k_blocks), seg++) {
                 const unsigned b = seg & 1;
+                const int64_t from_k = (int64_t)(at.k0 + k0) * kBlock, to_k = (int64_t)(at.k0 + segment_end(k0, k_blocks)) * kBlock;
+                const float gain = segment_gain<PB>(min(to_k, g.k_len) - from_k);
                 ok = __all_sync(0xffffffffu, mbar_wait(tfull + 8 * b, (seg >> 1) & 1, g.timeout_ns, stop));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                 for (int c = 0; c < kChunks; c++) {
                     const unsigned from = tmem + ((unsigned)(q * 32) << 16) + b * BN + column_of<EPI, kChunks>(half, c);
-                    tmem_add16(from, acc[c]), tmem_add16(from + 16, acc[c] + 16);
+                    tmem_add16(from, gain, acc[c]), tmem_add16(from + 16, gain, acc[c] + 16);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();

@@ -5,8 +5,8 @@ fp32, `eps / 2`):
   operands  each carries 22 bits (error 2^-22 of the value: hi rounds to 2^-11, lo to 2^-11 of that) and lo*lo is
             dropped (2^-22): 3 * 2^-22
   tensor    an accumulation rounds towards zero, off by one ulp at most, 2t of a partial sum that S bounds; 16 terms are
-            added at once, their alignment costs at most as much again: 4t per accumulation, 3 accumulations (products
-            of pieces) per 16 terms, at most 384 terms in a row
+            added at once, their alignment costs at most as much again: 4t per accumulation, and 0.28t are given back for
+            each on the average; 3 accumulations (products of pieces) per 16 terms, at most 384 terms in a row
   segments  one fp32 addition (t) per 256 terms
   scaling   exact (powers of two)
 """
@@ -22,7 +22,7 @@ T = np.finfo(np.float32).eps / 2
 
 def product_bound(k, s):
     steps = 3 * ((min(k, 384) + 15) // 16)
-    return (3 * 2.0 ** -22 + 4 * T * steps + T * ((k + 255) // 256)) * s
+    return (3 * 2.0 ** -22 + 4.28 * T * steps + T * ((k + 255) // 256)) * s
 
 
 class ByteBuf:
