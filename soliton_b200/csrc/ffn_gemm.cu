@@ -36,6 +36,7 @@ constexpr int kSmemBytes = kRingBytes + kEpiWarps * kTurnFloats * 4 + 256 + 1024
 // epilogue. At 4096 x 4096 x 1024 with GELU: 4 and 4 take 134 us, 6 and 6 112, 8 and 8 109 for a third more error.
 constexpr int kSegment = 4, kFirstSegments = 6;
 constexpr int kMaxStages = 4;
+constexpr unsigned long long kDrainNs = 2000000000ull;      // bound of the waits for a block's own copies and products at its end
 constexpr int kPlanSMs = 148;                               // how products are cut must not depend on the device
 constexpr int kGroupM = 8;                                  // row tiles that blocks walk side by side (reuse in L2)
 
@@ -510,12 +511,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                         if (j < nb) bulk_load(at_b + j * kBBlock, g.b.plane + (b_at[j] + (int64_t)kb * g.b.k_stride) * (int64_t)kBBlock, kBBlock, bar);
                 }
             }
-            if (!ok) {  // nothing may still be on its way into this block's shared memory when it ends
-                give_up(g, stop);
-                for (unsigned back = it < (unsigned)kStages ? it : (unsigned)kStages; back > 0; back--) {
-                    const unsigned i = it - back;
-                    mbar_wait(full + 8 * (i % kStages), (i / kStages) & 1, g.timeout_ns, nullptr);
-                }
+            if (!ok) give_up(g, stop);
+            // Nothing may still be on its way into this block's shared memory when it ends, whoever else has given up.
+            for (unsigned back = it < (unsigned)kStages ? it : (unsigned)kStages; back > 0; back--) {
+                const unsigned i = it - back;
+                mbar_wait(full + 8 * (i % kStages), (i / kStages) & 1, kDrainNs, nullptr);
             }
         }
         if (warp == 1 && lane == 0 && rank == 0) {
@@ -556,11 +556,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                     if (ok) mma_commit<CTAS>(tfull + 8 * buf);
                 }
             }
-            if (!ok) {
-                give_up(g, stop);
-                mma_commit<CTAS>(drained);
-                mbar_wait(drained, 0, g.timeout_ns, nullptr);
-            }
+            if (!ok) give_up(g, stop);
+            mma_commit<CTAS>(drained);  // nor may products still be reading it, or writing tensor memory
+            mbar_wait(drained, 0, kDrainNs, nullptr);
         }
         if (CTAS == 2 && warp == 1 && lane == 0 && rank == 1) {
             const unsigned there = remote(peer_full, 0);
