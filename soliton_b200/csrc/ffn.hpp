@@ -133,7 +133,8 @@ struct GemmPlan {
     size_t partial_bytes;
     int counters;
 };
-GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks);
+// store: a plain product (EPI_STORE)
+GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks, bool store);
 
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t st);
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);

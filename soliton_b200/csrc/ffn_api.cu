@@ -59,7 +59,7 @@ size_t carve(Scratch& s, void* base, int64_t m, int64_t n, int64_t k, int weight
     s.x = c.take((size_t)(mb * kb) * block);
     s.w = c.take((size_t)(weights * nb * kb) * block);
     if (backward) {
-        const GemmPlan dx = gemm_plan(mb, kb, weights * nb), dw = gemm_plan(weights * nb, kb, mb), half = gemm_plan(nb, kb, mb);
+        const GemmPlan dx = gemm_plan(mb, kb, weights * nb, true), dw = gemm_plan(weights * nb, kb, mb, true), half = gemm_plan(nb, kb, mb, true);
         const int dw_counters = dw.counters > half.counters ? dw.counters : half.counters;
         s.y = c.take((size_t)(weights * mb * nb) * block);
         s.exps = reinterpret_cast<int*>(c.take(kMaxPlanes * sizeof(int)));
@@ -72,7 +72,7 @@ size_t carve(Scratch& s, void* base, int64_t m, int64_t n, int64_t k, int weight
         partial = dx.partial_bytes > dw.partial_bytes ? dx.partial_bytes : dw.partial_bytes;
         if (half.partial_bytes > partial) partial = half.partial_bytes;  // one of the gated pair's weights alone
     } else {
-        const GemmPlan p = gemm_plan(mb, weights * nb, kb);
+        const GemmPlan p = gemm_plan(mb, weights * nb, kb, false);
         s.row_factor = reinterpret_cast<float*>(c.take((size_t)(mb * kBlock) * sizeof(float)));
         s.col_factor = reinterpret_cast<float*>(c.take((size_t)(nb * kBlock) * sizeof(float)));
         s.col_factor2 = weights == 2 ? reinterpret_cast<float*>(c.take((size_t)(nb * kBlock) * sizeof(float))) : nullptr;
@@ -266,7 +266,7 @@ void gradients(Op& op, const Scratch& s, bool x_ck8, float* dx, float* dw, float
         const bool both = dw && dw2;
         const char* y = s.y + (halves == 2 && !dw ? nb * (int64_t)(2 * kImageBytes) : 0);
         GemmArgs g = product(op, s);
-        g.counters += gemm_plan(mb, kb, width).counters;  // behind dx's
+        g.counters += gemm_plan(mb, kb, width, true).counters;  // behind dx's
         g.a = mn_major(y, both ? width : nb, width, PLANE_Y), g.b = mn_major(s.x, kb, kb, PLANE_X);
         g.k_blocks = (int)mb, g.k_len = m, g.rows = n, g.cols = k, g.out = dw ? dw : dw2;
         if (both) g.split = nb * kBlock, g.out2 = dw2;

@@ -395,17 +395,24 @@ __device__ __forceinline__ Unit unit_at(int u, const GemmArgs& g) {
     return r;
 }
 
-// A warp's sums over one slice of a tile go to memory; the warp that comes last adds up all slices, in their order, and has
-// the tile (true). Nobody waits. `who` of `warps`: the part of the tile.
+// Where a warp's sums over a slice lie in memory: 32 rows of CHUNKS x 32 columns, four columns of a lane's row together.
+// `who` of `warps`: the part of the tile.
 template <int CHUNKS>
-__device__ __forceinline__ bool add_slices(const GemmArgs& g, float (&acc)[CHUNKS][32], int slice, int warps, int who, int lane) {
-    constexpr int kFloats = CHUNKS * 32 * 32;
-    const auto place = [&](int s) { return reinterpret_cast<float4*>(g.partial) + ((int64_t)s * warps + who) * (kFloats / 4) + lane; };
-    float4* mine = place(slice);
+__device__ __forceinline__ float4* slice_place(float* partial, int slice, int warps, int who, int lane) {
+    return reinterpret_cast<float4*>(partial) + ((int64_t)slice * warps + who) * (CHUNKS * 256) + lane;
+}
+template <int CHUNKS>
+__device__ __forceinline__ void put_slice(const GemmArgs& g, const float (&acc)[CHUNKS][32], int slice, int warps, int who, int lane) {
+    float4* to = slice_place<CHUNKS>(g.partial, slice, warps, who, lane);
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) __stcg(mine + (c * 8 + i) * 32, make_float4(acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]));
+        for (int i = 0; i < 8; i++) __stcg(to + (c * 8 + i) * 32, make_float4(acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]));
+}
+// The sums go to memory; the warp that comes last adds up all slices, in their order, and has the tile (true). Nobody waits.
+template <int CHUNKS>
+__device__ __forceinline__ bool add_slices(const GemmArgs& g, float (&acc)[CHUNKS][32], int slice, int warps, int who, int lane) {
+    put_slice(g, acc, slice, warps, who, lane);
     __threadfence();
     __syncwarp();
     int before = 0;
@@ -420,7 +427,7 @@ __device__ __forceinline__ bool add_slices(const GemmArgs& g, float (&acc)[CHUNK
         for (int i = 0; i < 32; i++) acc[c][i] = 0.0f;
 #pragma unroll 1
     for (int s = 0; s < g.slices; s++) {
-        const float4* from = place(first + s);
+        const float4* from = slice_place<CHUNKS>(g.partial, first + s, warps, who, lane);
 #pragma unroll
         for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
@@ -430,6 +437,57 @@ __device__ __forceinline__ bool add_slices(const GemmArgs& g, float (&acc)[CHUNK
             }
     }
     return true;
+}
+// With many slices the warps that come last sit on few SMs and have much to read (30 k of 69 k cycles at eight slices of
+// 768 x 768 over 8192 terms); plain products leave it to a kernel of its own then.
+constexpr int kManySlices = 5;
+__device__ __host__ constexpr bool later(int epi, int slices) { return epi == EPI_STORE && slices >= kManySlices; }
+
+// Undoes both planes' scaling, in two steps that cannot overflow before the result does.
+__device__ __forceinline__ void plane_scales(const GemmArgs& g, float& s1, float& s2) {
+    const int e = g.exps[g.a.exp_id] + g.exps[g.b.exp_id] - 30;
+    s1 = exp2f((float)(e / 2)), s2 = exp2f((float)(e - e / 2));
+}
+// The 32 rows of tile row m, block `rank` of the team, that quadrant q covers, and how many of them exist.
+template <int CTAS, int EPI>
+__device__ __forceinline__ Piece rows_of(const GemmArgs& g, int m, int rank, int q) {
+    Piece p;
+    p.row0 = (int64_t)(m * CTAS + rank) * BM + q * 32;
+    int64_t left = g.rows - p.row0;
+    if (EPI == EPI_STORE && p.row0 >= g.split) left += g.split;
+    p.rows = left < 0 ? 0 : left < 32 ? (int)left : 32;
+    return p;
+}
+
+// The slices' sums, a warp per 32 x 32 results: grid over tiles, then parts of a tile, then chunks.
+template <int CTAS>
+__global__ void __launch_bounds__(32 * kEpiWarps) k_slices(const __grid_constant__ GemmArgs g) {
+    constexpr int kChunks = 2 * CTAS, kWarps = CTAS * kEpiWarps;
+    __shared__ float turn_buf[kEpiWarps][kTurnFloats];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    stream_next();
+    stream_wait();
+    const int unit = (int)blockIdx.x * kEpiWarps + warp, c = unit % kChunks, who = unit / kChunks % kWarps, tile = unit / (kChunks * kWarps);
+    const Unit at = unit_at(g.whole + tile * g.slices, g);
+    const int rank = who / kEpiWarps, q = who & 3, half = who / 4 % 2;
+    Piece p = rows_of<CTAS, EPI_STORE>(g, at.m, rank, q);
+    p.col0 = (int64_t)at.n * 128 * CTAS + (half * kChunks + c) * 32;
+    if (p.rows == 0 || p.col0 >= g.cols) return;
+    float v[32], s1, s2;
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = 0.0f;
+#pragma unroll 2
+    for (int s = 0; s < g.slices; s++) {
+        const float4* from = slice_place<kChunks>(g.partial, tile * g.slices + s, kWarps, who, lane) + c * 256;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float4 x = __ldcg(from + i * 32);
+            v[4 * i] += x.x, v[4 * i + 1] += x.y, v[4 * i + 2] += x.z, v[4 * i + 3] += x.w;
+        }
+    }
+    plane_scales(g, s1, s2);
+    if (g.wide && p.col0 + 32 <= g.cols) finish_wide<EPI_STORE>(g, v, v, p, s1, s2, turn_buf[warp], lane);
+    else finish_any<EPI_STORE>(g, v, v, p, s1, s2, turn_buf[warp], lane);
 }
 
 // CTAS = 1: a block per tile of 128 x 128. CTAS = 2: a pair of blocks (a cluster) per tile of 256 x 256: each holds 128 rows of A
@@ -582,10 +640,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
         const int q = warp & 3, half = (warp >> 2) - 1;  // a warp reads the 32 rows of tensor memory that its number mod 4 gives
         float* buf = turn + (warp - 4) * kTurnFloats;
         float s1 = 0.0f, s2 = 0.0f;
-        if (EPI == EPI_STORE) {  // undo both planes' scaling, in two steps that cannot overflow before the result does
-            const int e = g.exps[g.a.exp_id] + g.exps[g.b.exp_id] - 30;
-            s1 = exp2f((float)(e / 2)), s2 = exp2f((float)(e - e / 2));
-        }
+        if (EPI == EPI_STORE) plane_scales(g, s1, s2);
         unsigned seg = 0;
         bool ok = true;
         for (int t = team; ok && t < units; t += teams) {
@@ -622,13 +677,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
                 }
             }
             if (!ok) break;
-            if (at.slice >= 0 && !add_slices(g, acc, at.slice, CTAS * kEpiWarps, rank * kEpiWarps + warp - 4, lane)) continue;
-            Piece p;
-            p.row0 = (int64_t)(at.m * CTAS + rank) * BM + q * 32;
-            int64_t left = g.rows - p.row0;
-            if (EPI == EPI_STORE && p.row0 >= g.split) left += g.split;
-            p.rows = left < 0 ? 0 : left < 32 ? (int)left : 32;
+            Piece p = rows_of<CTAS, EPI>(g, at.m, rank, q);
             if (p.rows == 0) continue;
+            if (at.slice >= 0) {
+                const int who = rank * kEpiWarps + warp - 4;
+                if (later(EPI, g.slices)) {
+                    put_slice(g, acc, at.slice, CTAS * kEpiWarps, who, lane);
+                    continue;
+                }
+                if (!add_slices(g, acc, at.slice, CTAS * kEpiWarps, who, lane)) continue;
+            }
             if (EPI != EPI_STORE) s1 = g.row_factor[p.row0 + lane];  // whole blocks of factors exist
             // In place and in a loop that moves the next chunk up: registers are short, and so should the code be, which runs
             // once per tile and is bound by fetching it when it is long (150 k cycles a tile for four chunks in a row).
@@ -661,24 +719,26 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
 // Estimated cycles of a way of cutting: rounds of whole tiles, then rounds of slices. A k-block takes a pair 1,750 cycles,
 // bound by what the L2 delivers, and a single block, which fetches as much for half the work, the same when most SMs run,
 // 1,100 when few do; a tile's first fetches and what of its epilogue nothing covers 9,000 (6,000 single); a slice's sums
-// are written once and read once, 3,000 each (1,500).
-static double cut_cost(int ctas, int64_t tiles, int64_t k_blocks, int64_t slices) {
+// are written once and read once, 3,000 each (1,500); where a kernel of its own reads them,
+// a tenth of that, and 8,000 for it to come and go.
+static double cut_cost(int ctas, int64_t tiles, int64_t k_blocks, int64_t slices, bool store) {
     const int64_t teams = kPlanSMs / ctas, rounds = tiles / teams, rest = tiles % teams;
     const int64_t busy = rounds > 0 ? kPlanSMs : rest * slices * ctas;
     const double block = ctas == 2 || busy > 100 ? 1750 : 1100, tile = ctas == 2 ? 9000 : 6000, slice = ctas == 2 ? 3000 : 1500;
     double t = (double)rounds * (block * (double)k_blocks + tile);
     if (rest) t += (double)((rest * slices + teams - 1) / teams) * (block * (double)((k_blocks + slices - 1) / slices) + tile);
+    if (later(store ? EPI_STORE : EPI_LINEAR, (int)slices)) return t + slice * (1.0 + 0.1 * (double)slices) + 8000;
     return slices > 1 ? t + slice * (double)(1 + slices) : t;
 }
 
-GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks) {
+GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks, bool store) {
     GemmPlan best{};
     double least = 0;
     for (int ctas = 1; ctas <= 2; ctas++) {
         const int64_t mt = (m_blocks + 2 * ctas - 1) / (2 * ctas), nt = (n_blocks + 2 * ctas - 1) / (2 * ctas), tiles = mt * nt;
         const int64_t teams = kPlanSMs / ctas, rest = tiles % teams;
         for (int64_t s = 1; s <= k_blocks && s <= 16 && (s == 1 || rest * s <= 3 * teams); s++) {
-            const double t = cut_cost(ctas, tiles, k_blocks, s);
+            const double t = cut_cost(ctas, tiles, k_blocks, s, store);
             if (best.ctas && t >= least) continue;
             least = t;
             best.ctas = ctas, best.m_tiles = (int)mt, best.n_tiles = (int)nt;
@@ -695,11 +755,14 @@ static cudaError_t launch_one(const GemmArgs& g, int sm_count, cudaStream_t st) 
     static const cudaError_t ready = cudaFuncSetAttribute(k_gemm<CTAS, PB, AMN, BMN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (ready != cudaSuccess) return ready;
     const int units = g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices, teams = sm_count / CTAS;
-    return launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
+    const cudaError_t rc = launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
+    if (rc != cudaSuccess || !later(EPI, g.slices)) return rc;
+    const int cut = g.m_tiles * g.n_tiles - g.whole;  // CTAS x kEpiWarps parts of 2 CTAS chunks each, kEpiWarps to a block
+    return launch_early(k_slices<CTAS>, dim3((unsigned)(cut * CTAS * 2 * CTAS)), 32 * kEpiWarps, 0, st, 1, g);
 }
 template <int PB, bool AMN, bool BMN, int EPI>
 static cudaError_t launch_sized(GemmArgs& g, int sm_count, cudaStream_t st) {
-    const GemmPlan p = gemm_plan(g.a.mn_blocks, EPI == EPI_GATED ? 2 * (int64_t)g.gate_blocks : g.b.mn_blocks, g.k_blocks);
+    const GemmPlan p = gemm_plan(g.a.mn_blocks, EPI == EPI_GATED ? 2 * (int64_t)g.gate_blocks : g.b.mn_blocks, g.k_blocks, EPI == EPI_STORE);
     g.m_tiles = p.m_tiles, g.n_tiles = p.n_tiles, g.whole = p.whole, g.slices = p.slices;
     return p.ctas == 1 ? launch_one<1, PB, AMN, BMN, EPI>(g, sm_count, st) : launch_one<2, PB, AMN, BMN, EPI>(g, sm_count, st);
 }
