@@ -460,14 +460,15 @@ __device__ __forceinline__ Piece rows_of(const GemmArgs& g, int m, int rank, int
 }
 
 // The slices' sums, a warp per 32 x 32 results: grid over tiles, then parts of a tile, then chunks.
+constexpr int kSliceWarps = 4;
 template <int CTAS>
-__global__ void __launch_bounds__(32 * kEpiWarps) k_slices(const __grid_constant__ GemmArgs g) {
+__global__ void __launch_bounds__(32 * kSliceWarps) k_slices(const __grid_constant__ GemmArgs g) {
     constexpr int kChunks = 2 * CTAS, kWarps = CTAS * kEpiWarps;
-    __shared__ float turn_buf[kEpiWarps][kTurnFloats];
+    __shared__ alignas(16) float turn_buf[kSliceWarps][kTurnFloats];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     stream_next();
     stream_wait();
-    const int unit = (int)blockIdx.x * kEpiWarps + warp, c = unit % kChunks, who = unit / kChunks % kWarps, tile = unit / (kChunks * kWarps);
+    const int unit = (int)blockIdx.x * kSliceWarps + warp, c = unit % kChunks, who = unit / kChunks % kWarps, tile = unit / (kChunks * kWarps);
     const Unit at = unit_at(g.whole + tile * g.slices, g);
     const int rank = who / kEpiWarps, q = who & 3, half = who / 4 % 2;
     Piece p = rows_of<CTAS, EPI_STORE>(g, at.m, rank, q);
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(32 * kEpiWarps) k_slices(const __grid_constant
     float v[32], s1, s2;
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = 0.0f;
-#pragma unroll 2
+#pragma unroll 4
     for (int s = 0; s < g.slices; s++) {
         const float4* from = slice_place<kChunks>(g.partial, tile * g.slices + s, kWarps, who, lane) + c * 256;
 #pragma unroll
@@ -757,8 +758,8 @@ static cudaError_t launch_one(const GemmArgs& g, int sm_count, cudaStream_t st) 
     const int units = g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices, teams = sm_count / CTAS;
     const cudaError_t rc = launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
     if (rc != cudaSuccess || !later(EPI, g.slices)) return rc;
-    const int cut = g.m_tiles * g.n_tiles - g.whole;  // CTAS x kEpiWarps parts of 2 CTAS chunks each, kEpiWarps to a block
-    return launch_early(k_slices<CTAS>, dim3((unsigned)(cut * CTAS * 2 * CTAS)), 32 * kEpiWarps, 0, st, 1, g);
+    const int cut = g.m_tiles * g.n_tiles - g.whole;  // of CTAS x kEpiWarps parts of 2 CTAS chunks each
+    return launch_early(k_slices<CTAS>, dim3((unsigned)(cut * CTAS * kEpiWarps * 2 * CTAS / kSliceWarps)), 32 * kSliceWarps, 0, st, 1, g);
 }
 template <int PB, bool AMN, bool BMN, int EPI>
 static cudaError_t launch_sized(GemmArgs& g, int sm_count, cudaStream_t st) {

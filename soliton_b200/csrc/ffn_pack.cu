@@ -39,19 +39,21 @@ __device__ __forceinline__ unsigned finite_bits(float x) {
 }
 __device__ __forceinline__ unsigned finite_byte(unsigned byte) { return byte == 255u ? 0u : byte; }
 
-__global__ void __launch_bounds__(kThreads) k_amax(AmaxArgs a) {
+// SAMPLED: some of the tensors are.
+template <bool SAMPLED>
+__global__ void __launch_bounds__(kThreads) k_amax(const __grid_constant__ AmaxArgs a) {
     stream_next();
     stream_wait();
     const int s = blockIdx.y;
-    const AmaxSlot t = a.slot[s];
+    const AmaxSlot& t = a.slot[s];
     if ((int)blockIdx.x >= t.parts) return;
     unsigned top = 0;
     const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, step = (int64_t)t.parts * kThreads;
-    if (a.tops && blockIdx.x == 0 && s == 0 && threadIdx.x < kMaxPlanes) a.tops[threadIdx.x] = 0;
+    if (SAMPLED && blockIdx.x == 0 && s == 0 && threadIdx.x < kMaxPlanes) a.tops[threadIdx.x] = 0;
     if (t.is_ck8) {
         const unsigned char* p = static_cast<const unsigned char*>(t.p);
         for (int64_t i = at; i < t.n; i += step) top = max(top, finite_byte(p[i]));
-    } else if (t.sampled) {  // a 16-byte word a thread of 4 KiB in every 64; only where a tensor has many of those
+    } else if (SAMPLED && t.sampled) {  // a 16-byte word a thread of 4 KiB in every 64; only where a tensor has many of those
         const float4* w = reinterpret_cast<const float4*>((reinterpret_cast<uintptr_t>(t.p) + 15) & ~(uintptr_t)15);
         const int64_t strips = (t.n - 4) / 16384;
 #pragma unroll 4
@@ -397,7 +399,9 @@ cudaError_t launch_rows(const RowArgs& a, cudaStream_t st) {
 cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {
     int most = 1;
     for (int s = 0; s < a.slots; s++) most = most > a.slot[s].parts ? most : a.slot[s].parts;
-    return launch_early(k_amax, dim3((unsigned)most, (unsigned)a.slots), kThreads, 0, st, 1, a);
+    bool sampled = false;
+    for (int s = 0; s < a.slots; s++) sampled |= a.slot[s].sampled != 0;
+    return launch_early(sampled ? k_amax<true> : k_amax<false>, dim3((unsigned)most, (unsigned)a.slots), kThreads, 0, st, 1, a);
 }
 
 static bool gated(const PackArgs& a) { return a.job[0].kind == PACK_GATED; }  // it comes first
