@@ -238,12 +238,16 @@ int slb_adamw_step_static(int nseg, float* const* p, const float* const* g, floa
  * value per feature out. Activations: 0 none, 1 GELU (exact, through erf), 2 SiLU. Work goes to the legacy default
  * stream (so a call cannot be captured into a graph); nothing is kept from one call for the next; the same inputs give
  * the same bits. Results 0, -1 (sticky error set: 12 bad argument, 13 cpu, 14 device not initialised, 2 launch), -2 out
- * of memory. m = 0 is allowed: no output rows, and gradients of weights and biases are zero.
+ * of memory. m = 0 is allowed: no output rows, and gradients of weights and biases are zero; k and n are at least 1.
  *
- * Products are fp32-class: operands carry 22 bits wherever a value is within 2^17 of its tensor's largest, and an
- * absolute error of 2^-40 of the largest below that; sums are fp32. An infinity or NaN in an operand makes the outputs
- * that depend on it non-finite, a NaN where fp32 might still have an infinity. Outputs must not overlap inputs, but for
- * `y` = `residual` exactly.
+ * Products are fp32-class. Operands are cut into two fp16 pieces under a power of two as scale, of each row in the forward
+ * calls, of the whole tensor in the backward calls: 22 bits for values within 2^17 of the largest under the same scale and
+ * an absolute error of 2^-40 of it below (2^11 and 2^-34 for gradients of tensors that exceed 100 MiB together). Sums are
+ * fp32 and on random data as near to the exact ones as fp32 arithmetic's (0.7e-6 of the norm over 1024 terms); sums that
+ * fp32 would have exact may be off by some 2^-20. An infinity or NaN in an operand makes the outputs that depend on it
+ * non-finite, a NaN where fp32 might still have an infinity. Outputs must not overlap inputs, but for `y` = `residual`
+ * exactly. Which of the gradients are asked for does not change their bits, but that the gated block's two weights take
+ * other sums together than one alone.
  *
  * The `slb_` calls take their scratch from the pool and give it back before they return, on meta as on cuda, so a dry
  * run plans it; the `slb_cuda_` calls (cuda only) are given it: 256-byte aligned, at least what the `_scratch_bytes`
