@@ -8,7 +8,7 @@ from tests.ffn_util import T, ByteBuf, Out, close
 from tests.gpu_util import CUDA, DevBuf, check_ok
 
 pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("cuda")]
-SHAPES = [(1, 1), (1, 31), (3, 32), (7, 33), (5, 64), (1, 4096), (64, 127), (129, 2305), (300, 512)]
+SHAPES = [(1, 1), (1, 31), (3, 32), (7, 33), (5, 64), (1, 4096), (64, 127), (129, 2305), (300, 512), (40, 65), (61, 34)]
 
 
 def special(rows, cols):
