@@ -70,38 +70,48 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __re
     }
 }
 
-// Any columns, any alignment: a warp per group, a lane per column, four groups of a warp in flight.
-constexpr int kAheadAny = 4;
-struct Spot {
-    int64_t at;         // element, or -1 where the lane has none
-    int64_t group;
-};
-__device__ __forceinline__ void find_spots(Spot (&s)[kAheadAny], int64_t rows, int64_t cols) {
+// Any columns, any alignment: a warp takes 128 columns of a row, four groups, a lane four of them; kStrips such strips in
+// flight. QUADS: rows and buffers allow the four at once. (8192 x 4097: 86 us with a warp per group.)
+constexpr int kStrips = 2;
+template <bool QUADS, class Index>
+__global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__ x, char* __restrict__ ck, int64_t rows, Index cols) {
     const int lane = threadIdx.x & 31;
-    const int64_t groups = ck8_groups(cols), first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAheadAny;
-    int64_t row = first / groups, g = first - row * groups;
-#pragma unroll
-    for (int i = 0; i < kAheadAny; i++) {
-        s[i].group = first + i;
-        s[i].at = row < rows && g * kGroup + lane < cols ? row * cols + g * kGroup + lane : -1;
-        if (++g == groups) g = 0, row++;
-    }
-}
-__global__ void __launch_bounds__(kThreads) k_ck8_save(const float* __restrict__ x, char* __restrict__ ck, int64_t rows, int64_t cols) {
-    const int lane = threadIdx.x & 31;
-    const int64_t total = rows * ck8_groups(cols);
+    const Index strips = (cols + 127) / 128, first = ((Index)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kStrips;
     unsigned char* eb = reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols);
-    Spot s[kAheadAny];
-    float v[kAheadAny];
-    find_spots(s, rows, cols);
+    Index row = first / strips, strip = first - row * strips;
+    float v[kStrips][4];
+    int64_t at[kStrips], group[kStrips];
+    int have[kStrips];
 #pragma unroll
-    for (int i = 0; i < kAheadAny; i++) v[i] = s[i].at >= 0 ? __ldcs(x + s[i].at) : 0.0f;
+    for (int i = 0; i < kStrips; i++) {
+        const Index col = strip * 128 + lane * 4;
+        have[i] = (int64_t)row >= rows || col >= cols ? 0 : cols - col < 4 ? (int)(cols - col) : 4;
+        at[i] = (int64_t)row * cols + col, group[i] = (int64_t)row * ck8_groups(cols) + col / kGroup;
+        if (QUADS && have[i] == 4) {
+            const float4 w = __ldcs(reinterpret_cast<const float4*>(x + at[i]));
+            v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
+        } else {
 #pragma unroll
-    for (int i = 0; i < kAheadAny; i++) {
-        if (s[i].group >= total) break;
-        const unsigned byte = ck8_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
-        if (s[i].at >= 0) ck[s[i].at] = (char)ck8_quantise(v[i], byte);
-        if (lane == 0) eb[s[i].group] = (unsigned char)byte;
+            for (int j = 0; j < 4; j++) v[i][j] = j < have[i] ? __ldg(x + at[i] + j) : 0.0f;
+        }
+        if (++strip == strips) strip = 0, row++;
+    }
+#pragma unroll
+    for (int i = 0; i < kStrips; i++) {
+        unsigned top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const unsigned byte = ck8_exponent(top), q = ck8_quantise4(v[i][0], v[i][1], v[i][2], v[i][3], byte);
+        if (QUADS && have[i] == 4) {
+            *reinterpret_cast<unsigned*>(ck + at[i]) = q;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j < have[i]) ck[at[i] + j] = (char)(q >> (8 * j));
+        }
+        if ((lane & 7) == 0 && have[i] > 0) eb[group[i]] = (unsigned char)byte;
     }
 }
 
@@ -154,25 +164,31 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_flat(const uint2* __restr
     }
 }
 
+// Any columns, any alignment: a warp per group, a lane per column, four groups of a warp in flight.
+constexpr int kAheadAny = 4;
 template <bool GELU_BWD>
 __global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ ck, const float* __restrict__ dy, float* __restrict__ out, int64_t rows,
                                                        int64_t cols) {
+    const int lane = threadIdx.x & 31;
+    const int64_t groups = ck8_groups(cols), first = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kAheadAny;
     const unsigned char* eb = reinterpret_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols);
-    Spot s[kAheadAny];
+    int64_t row = first / groups, g = first - row * groups, at[kAheadAny];
     float d[kAheadAny];
     int q[kAheadAny];
     unsigned byte[kAheadAny];
-    find_spots(s, rows, cols);
 #pragma unroll
-    for (int i = 0; i < kAheadAny; i++)
-        if (s[i].at >= 0) {
-            q[i] = (signed char)__ldg(ck + s[i].at);
-            byte[i] = __ldg(eb + s[i].group);
-            if (GELU_BWD) d[i] = __ldcs(dy + s[i].at);
+    for (int i = 0; i < kAheadAny; i++) {
+        at[i] = row < rows && g * kGroup + lane < cols ? row * cols + g * kGroup + lane : -1;
+        if (at[i] >= 0) {
+            q[i] = (signed char)__ldg(ck + at[i]);
+            byte[i] = __ldg(eb + first + i);
+            if (GELU_BWD) d[i] = __ldcs(dy + at[i]);
         }
+        if (++g == groups) g = 0, row++;
+    }
 #pragma unroll
     for (int i = 0; i < kAheadAny; i++)
-        if (s[i].at >= 0) out[s[i].at] = read_value<GELU_BWD>((float)q[i] * ck8_step(byte[i]), GELU_BWD ? d[i] : 0.0f);
+        if (at[i] >= 0) out[at[i]] = read_value<GELU_BWD>((float)q[i] * ck8_step(byte[i]), GELU_BWD ? d[i] : 0.0f);
 }
 
 static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -188,8 +204,18 @@ cudaError_t launch_ck8_save(const float* x, char* ck, int64_t rows, int64_t cols
     if (wide(cols, ck, x, nullptr))
         k_ck8_save_wide<<<wide_grid(rows, cols), kThreads, 0, st>>>(reinterpret_cast<const float4*>(x), reinterpret_cast<unsigned*>(ck),
                                                                   reinterpret_cast<unsigned char*>(ck) + ck8_exp_offset(rows, cols), rows * cols / 4);
-    else
-        k_ck8_save<<<any_grid(rows, cols), kThreads, 0, st>>>(x, ck, rows, cols);
+    else {
+        const int64_t warps = (rows * ((cols + 127) / 128) + kStrips - 1) / kStrips;
+        const unsigned grid = (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32));
+        const bool quads = cols % 4 == 0 && flat(ck, x, nullptr);
+        if (rows * ((cols + 127) / 128) < (int64_t(1) << 30)) {
+            if (quads) k_ck8_save<true, unsigned><<<grid, kThreads, 0, st>>>(x, ck, rows, (unsigned)cols);
+            else k_ck8_save<false, unsigned><<<grid, kThreads, 0, st>>>(x, ck, rows, (unsigned)cols);
+        } else {
+            if (quads) k_ck8_save<true, int64_t><<<grid, kThreads, 0, st>>>(x, ck, rows, cols);
+            else k_ck8_save<false, int64_t><<<grid, kThreads, 0, st>>>(x, ck, rows, cols);
+        }
+    }
     return cudaPeekAtLastError();
 }
 template <bool GELU_BWD>
