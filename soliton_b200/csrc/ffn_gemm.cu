@@ -374,17 +374,19 @@ __device__ __forceinline__ int segment_end(int k0, int k_blocks) {
 }
 
 // What a team takes up at a time: a tile, or a slice of one along K. Tiles that would leave most teams idle in the last
-// round are cut so that every team has a part.
+// round are cut so that every team has a part -- and come first, so that what joining them costs runs under the products of
+// whole tiles.
 struct Unit {
     int m, n, k0, k1, slice;        // slice: of all, -1 for a whole tile
 };
 __device__ __forceinline__ int units_of(const GemmArgs& g) { return g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices; }
 __device__ __forceinline__ Unit unit_at(int u, const GemmArgs& g) {
     Unit r;
-    int t = u;
+    const int cut = (g.m_tiles * g.n_tiles - g.whole) * g.slices;
+    int t = u - cut;
     r.slice = -1, r.k0 = 0, r.k1 = g.k_blocks;
-    if (u >= g.whole) {
-        r.slice = u - g.whole;
+    if (u < cut) {
+        r.slice = u;
         const int s = r.slice % g.slices;
         t = g.whole + r.slice / g.slices;
         r.k0 = (int)((int64_t)g.k_blocks * s / g.slices), r.k1 = (int)((int64_t)g.k_blocks * (s + 1) / g.slices);
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(32 * kSliceWarps) k_slices(const __grid_consta
     stream_next();
     stream_wait();
     const int unit = (int)blockIdx.x * kSliceWarps + warp, c = unit % kChunks, who = unit / kChunks % kWarps, tile = unit / (kChunks * kWarps);
-    const Unit at = unit_at(g.whole + tile * g.slices, g);
+    const Unit at = unit_at(tile * g.slices, g);
     const int rank = who / kEpiWarps, q = who & 3, half = who / 4 % 2;
     Piece p = rows_of<CTAS, EPI_STORE>(g, at.m, rank, q);
     p.col0 = (int64_t)at.n * 128 * CTAS + (half * kChunks + c) * 32;

@@ -286,3 +286,32 @@ def test_out_of_memory_is_reported():
     finally:
         lib.sl_set_limit(CUDA, 0)
     check_ok()
+
+
+def test_checkpoint_of_more_than_2_30_rows():
+    rows = (1 << 30) + 5
+    x, ck = lib.sl_alloc(CUDA, 4 * rows), lib.sl_alloc(CUDA, lib.slb_ck8_bytes(rows, 1))
+    assert x and ck
+    lib.sl_fill(CUDA, x, rows, 3.0)
+    tail = np.array([-1.0, 2.0 ** -20, 127.0, 128.0, 0.0], np.float32)
+    lib.sl_from_host(CUDA, x + 4 * (rows - 5), tail.ctypes.data, tail.nbytes)
+    assert lib.slb_ck8_save(CUDA, x, ck, rows, 1) == 0
+    q, eb = ops.ck8_save(np.concatenate([np.full(3, 3.0, np.float32), tail])[:, None])
+    got = np.empty(8, np.uint8)
+    for first in (0, (1 << 29) + 1, rows - 8):
+        lib.sl_to_host(CUDA, got.ctypes.data, ck + first, 8)
+        np.testing.assert_array_equal(got.view(np.int8)[:3], q[:3, 0])
+        if first == rows - 8:
+            np.testing.assert_array_equal(got.view(np.int8), q[:, 0])
+        lib.sl_to_host(CUDA, got.ctypes.data, ck + ops.ck8_exp_offset(rows, 1) + first, 8)
+        np.testing.assert_array_equal(got[:3], eb[:3, 0])
+        if first == rows - 8:
+            np.testing.assert_array_equal(got, eb[:, 0])
+    assert lib.slb_ck8_load(CUDA, ck, x, rows, 1) == 0
+    check_ok()
+    back = np.empty(5, np.float32)
+    lib.sl_to_host(CUDA, back.ctypes.data, x + 4 * (rows - 5), back.nbytes)
+    np.testing.assert_array_equal(back, ops.ck8_values(q, eb)[3:, 0].astype(np.float32))
+    lib.sl_free(CUDA, x, 4 * rows)
+    lib.sl_free(CUDA, ck, lib.slb_ck8_bytes(rows, 1))
+    lib.sl_empty_cache(CUDA)
