@@ -139,3 +139,37 @@ def test_same_bits_every_run(F, T, cuda):
     for (_, x, _), (_, y, _) in zip(a, b):
         for n in x:
             np.testing.assert_array_equal(x[n], y[n])
+
+
+@pytest.mark.gpu
+def test_an_arena_planned_on_meta_holds_a_step(F, T, cuda):
+    """Recorded on meta, packed, installed, and replayed on the GPU: operators' scratch, checkpoints and gradients all lie
+    in the one planned allocation, and the values are those of the plain pool."""
+    from soliton_b200 import arena
+    rng = np.random.default_rng(3)
+    host = [rng.standard_normal(s).astype(np.float32) for s in ((300, 128), (256, 128), (256, 128), (128, 256))]
+
+    def step(dev):
+        x, wg, wu, wd = (T.tensor(h, dev) for h in host)
+        h, g, u = F.gated(x, wg, wu, keep="ck8")
+        h8 = F.Checkpoint.save(h)
+        y = F.linear(h, wd, residual=x)
+        del h
+        dh, dwd, _ = F.linear_bwd(y, h8, wd, need=("x", "w"))
+        grads = F.gated_bwd(dh, F.Checkpoint.save(x), wg, wu, g, u, bias=False)[:3] + (dwd,)
+        return [t.numpy() for t in grads] if dev == "cuda" else None
+
+    T.empty_cache("cuda")
+    want = step("cuda")
+    plan = arena.plan(step)
+    T.empty_cache("cuda")
+    before = T.memory_stats("cuda")["reserved"]
+    arena.install(plan, "cuda")
+    try:
+        got = step("cuda")
+        arena.check("cuda")
+        assert T.memory_stats("cuda")["reserved"] - before == plan.bytes
+    finally:
+        arena.off("cuda")
+    for a, b in zip(got, want):
+        np.testing.assert_array_equal(a, b)
