@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(kThreads) k_ck8_save_wide(const float4* __rest
 }
 
 template <bool GELU_BWD>
-__device__ __forceinline__ float read_value(float v, float dy) { return GELU_BWD ? dy * act_grad(ACT_GELU, v) : v; }
+__device__ __forceinline__ Two read_values(const Two& v, const Two& dy) { return GELU_BWD ? mul2(dy, act_grad2(ACT_GELU, v)) : v; }
 
 template <bool GELU_BWD>
 __global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __restrict__ q, const unsigned char* __restrict__ eb, const float4* __restrict__ dy,
@@ -61,11 +61,9 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_wide(const unsigned* __re
         const int64_t at = first + i * kThreads;
         if (at >= quads) break;
         const float step = ck8_step(byte[i]);
-        float4 o;
-        o.x = read_value<GELU_BWD>(ck8_integer<0>(w[i]) * step, GELU_BWD ? d[i].x : 0.0f);
-        o.y = read_value<GELU_BWD>(ck8_integer<1>(w[i]) * step, GELU_BWD ? d[i].y : 0.0f);
-        o.z = read_value<GELU_BWD>(ck8_integer<2>(w[i]) * step, GELU_BWD ? d[i].z : 0.0f);
-        o.w = read_value<GELU_BWD>(ck8_integer<3>(w[i]) * step, GELU_BWD ? d[i].w : 0.0f);
+        const Two lo = read_values<GELU_BWD>(mul2(Two{ck8_integer<0>(w[i]), ck8_integer<1>(w[i])}, both(step)), GELU_BWD ? Two{d[i].x, d[i].y} : both(0.0f));
+        const Two hi = read_values<GELU_BWD>(mul2(Two{ck8_integer<2>(w[i]), ck8_integer<3>(w[i])}, both(step)), GELU_BWD ? Two{d[i].z, d[i].w} : both(0.0f));
+        const float4 o = make_float4(lo.x, lo.y, hi.x, hi.y);
         __stcs(out + at, o);
     }
 }
@@ -153,7 +151,11 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read_flat(const uint2* __restr
     o[0] = ck8_integer<0>(w.x), o[1] = ck8_integer<1>(w.x), o[2] = ck8_integer<2>(w.x), o[3] = ck8_integer<3>(w.x);
     o[4] = ck8_integer<0>(w.y), o[5] = ck8_integer<1>(w.y), o[6] = ck8_integer<2>(w.y), o[7] = ck8_integer<3>(w.y);
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = read_value<GELU_BWD>(o[i] * (i < first ? step0 : i < second ? step1 : step2), GELU_BWD ? d[i] : 0.0f);
+    for (int i = 0; i < 8; i += 2) {
+        const Two step = Two{i < first ? step0 : i < second ? step1 : step2, i + 1 < first ? step0 : i + 1 < second ? step1 : step2};
+        const Two r = read_values<GELU_BWD>(mul2(Two{o[i], o[i + 1]}, step), GELU_BWD ? Two{d[i], d[i + 1]} : both(0.0f));
+        o[i] = r.x, o[i + 1] = r.y;
+    }
     if (have == 8) {
         __stcs(reinterpret_cast<float4*>(out + at), make_float4(o[0], o[1], o[2], o[3]));
         __stcs(reinterpret_cast<float4*>(out + at) + 1, make_float4(o[4], o[5], o[6], o[7]));
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) k_ck8_read(const char* __restrict__ 
     }
 #pragma unroll
     for (int i = 0; i < kAheadAny; i++)
-        if (at[i] >= 0) out[at[i]] = read_value<GELU_BWD>((float)q[i] * ck8_step(byte[i]), GELU_BWD ? d[i] : 0.0f);
+        if (at[i] >= 0) out[at[i]] = read_values<GELU_BWD>(both((float)q[i] * ck8_step(byte[i])), both(GELU_BWD ? d[i] : 0.0f)).x;
 }
 
 static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

@@ -51,6 +51,9 @@ struct PackJob {
     const float* a;                 // the matrix, dy or dh
     const float *b, *c;             // pre, or g and u, in fp32 ...
     const void *b8, *c8;            // ... or as checkpoints; `b8` alone with PACK_CK8
+    const unsigned char *b_exp, *c_exp;  // their exponent bytes (set by launch_pack, like the next three)
+    int a_wide, b_wide, c_wide;     // eight values of a row at a multiple of eight may be read at once
+    int64_t groups;
     int64_t rows, cols;
     int row_blocks, col_blocks;     // of this matrix
     int row_stride;                 // blocks per block row of the plane
@@ -138,7 +141,7 @@ GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks, bool st
 
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t st);
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
-cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st);
+cudaError_t launch_pack(PackArgs& a, int sm_count, cudaStream_t st);
 // After a pack with sampled maxima: does planes again whose values went beyond what their exponent allows.
 cudaError_t launch_repack(const PackArgs& a, int sm_count, cudaStream_t st);
 // out[j] = the sum over `parts` of the block rows' column sums, in order; the same for a second matrix where given
@@ -208,38 +211,87 @@ __device__ __forceinline__ float ck8_integer(unsigned word) {
     return __uint_as_float(__byte_perm(word ^ 0x80808080u, 0x4b000000u, 0x7440 + J)) - 8388736.0f;
 }
 
-// exp and quotients to about two ulps; what an argument's rounding adds is relative to terms that vanish with it.
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+// Two floats an instruction.
+struct Two {
+    float x, y;
+};
+#define SLB_TWO(name, op)                                                                                                                            \
+    __device__ __forceinline__ Two name(const Two& a, const Two& b) {                                                                                \
+        Two r;                                                                                                                                       \
+        asm("{\n\t.reg .b64 a, b, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t" op " r, a, b;\n\tmov.b64 {%0, %1}, r;\n\t}"                        \
+            : "=f"(r.x), "=f"(r.y)                                                                                                                   \
+            : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));                                                                                               \
+        return r;                                                                                                                                    \
+    }
+SLB_TWO(mul2, "mul.rn.f32x2")
+SLB_TWO(add2, "add.rn.f32x2")
+#undef SLB_TWO
+__device__ __forceinline__ Two fma2(const Two& a, const Two& b, const Two& c) {
+    Two r;
+    asm("{\n\t.reg .b64 a, b, c, r;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 r, a, b, c;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ Two both(float v) { return Two{v, v}; }
+// 2^x and 1 / x to two ulps, subnormal results as zero.
+__device__ __forceinline__ Two exp2_2(const Two& v) {
+    Two r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ Two rcp2(const Two& v) {
+    Two r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+    return r;
+}
+
+// What an argument's rounding adds to an exponential is relative to terms that vanish with it.
+__device__ __forceinline__ Two sigmoid2(const Two& v) { return rcp2(add2(both(1.0f), exp2_2(mul2(v, both(-1.44269504f))))); }
 // Phi(v) and e = exp(-v^2 / 2). 1 - erf(z) = (a1 t + ... + a5 t^5) exp(-z^2) with t = 1 / (1 + p z), for z >= 0 (Abramowitz and
 // Stegun 7.1.26), is off by 1.5e-7 at most, which Phi halves: about an ulp of a value near one, at under half the
 // instructions of erff, whose cost showed (30 k cycles a tile of 128 x 256 against 24 k), and the derivative needs e anyway.
-__device__ __forceinline__ float normal_cdf(float v, float& e) {
-    const float z = fabsf(v) * 0.70710678f;
-    e = __expf(-0.5f * v * v);
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
-    // half the coefficients: tail = Phi(-|v|)
-    const float tail = e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
-    return v < 0.0f ? tail : 1.0f - tail;
+__device__ __forceinline__ Two normal_cdf2(const Two& v, Two& e) {
+    e = exp2_2(mul2(mul2(v, v), both(-0.72134752f)));
+    const Two t = rcp2(fma2(Two{fabsf(v.x), fabsf(v.y)}, both(0.23164189f), both(1.0f)));  // p / sqrt(2)
+    Two h = fma2(t, both(0.5307027145f), both(-0.7265760135f));                             // half the coefficients
+    h = fma2(t, h, both(0.7107068705f)), h = fma2(t, h, both(-0.142248368f)), h = fma2(t, h, both(0.127414796f));
+    const Two half = add2(both(0.5f), mul2(mul2(t, h), Two{-e.x, -e.y}));  // 1/2 - Phi(-|v|)
+    return add2(both(0.5f), Two{copysignf(half.x, v.x), copysignf(half.y, v.y)});
 }
-__device__ __forceinline__ float act_of(int act, float v) {
+__device__ __forceinline__ Two act2(int act, const Two& v) {
     if (act == ACT_GELU) {
-        float e;
-        return v * normal_cdf(v, e);
+        Two e;
+        return mul2(v, normal_cdf2(v, e));
     }
-    if (act == ACT_SILU) return v * sigmoid(v);
-    return v;
+    return act == ACT_SILU ? mul2(v, sigmoid2(v)) : v;
 }
-__device__ __forceinline__ float act_grad(int act, float v) {
+__device__ __forceinline__ Two act_grad2(int act, const Two& v) {
     if (act == ACT_GELU) {  // Phi(v) + v phi(v)
-        float e;
-        const float cdf = normal_cdf(v, e);
-        return fmaf(v * 0.39894228f, e, cdf);
+        Two e;
+        const Two cdf = normal_cdf2(v, e);
+        return fma2(mul2(v, both(0.39894228f)), e, cdf);
     }
     if (act == ACT_SILU) {
-        const float sig = sigmoid(v);
-        return sig * fmaf(v, 1.0f - sig, 1.0f);
+        const Two sig = sigmoid2(v);
+        return mul2(sig, fma2(v, Two{1.0f - sig.x, 1.0f - sig.y}, both(1.0f)));
     }
-    return 1.0f;
+    return both(1.0f);
+}
+// SiLU and its derivative share the sigmoid.
+__device__ __forceinline__ void act_and_grad2(int act, const Two& v, Two& value, Two& grad) {
+    if (act == ACT_GELU) {
+        Two e;
+        const Two cdf = normal_cdf2(v, e);
+        value = mul2(v, cdf), grad = fma2(mul2(v, both(0.39894228f)), e, cdf);
+    } else if (act == ACT_SILU) {
+        const Two sig = sigmoid2(v);
+        value = mul2(v, sig), grad = mul2(sig, fma2(v, Two{1.0f - sig.x, 1.0f - sig.y}, both(1.0f)));
+    } else {
+        value = v, grad = both(1.0f);
+    }
 }
 #endif
 

@@ -266,7 +266,10 @@ __device__ __forceinline__ void act_row(float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[i + j] = act_of(ACT, v[i + j]);
+        for (int j = 0; j < 8; j += 2) {
+            const Two r = act2(ACT, Two{v[i + j], v[i + j + 1]});
+            v[i + j] = r.x, v[i + j + 1] = r.y;
+        }
         // eight at a time: all 32 side by side would not fit the registers
         asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7]));
         if (i < 24)

@@ -119,11 +119,9 @@ __device__ __forceinline__ Eight load8(const float* p, int have, bool wide) {
     }
     return r;
 }
-// The same from a checkpoint: eight columns from a multiple of eight lie in one group.
-__device__ __forceinline__ Eight load8_ck(const void* ck, int64_t rows, int64_t cols, int64_t row, int64_t col, int have, bool wide) {
-    const signed char* q = static_cast<const signed char*>(ck) + row * cols + col;
-    const unsigned char* e = static_cast<const unsigned char*>(ck) + ck8_exp_offset(rows, cols) + row * ck8_groups(cols) + col / kGroup;
-    const float step = ck8_step(__ldg(e));
+// The same from a checkpoint, whose eight columns from a multiple of eight lie in one group.
+__device__ __forceinline__ Eight load8_ck(const signed char* q, const unsigned char* exp, int have, bool wide) {
+    const float step = ck8_step(__ldg(exp));
     Eight r;
     if (wide && have == 8) {
         const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
@@ -140,10 +138,11 @@ __device__ __forceinline__ void split8(const Eight& x, float scale, uint4& hi, u
     unsigned h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float a = x.v[2 * i] * scale, b = x.v[2 * i + 1] * scale;
-        const __half2 p = __floats2half2_rn(a, b);
+        const Two t = mul2(Two{x.v[2 * i], x.v[2 * i + 1]}, both(scale));
+        const __half2 p = __floats2half2_rn(t.x, t.y);
         const float2 f = __half22float2(p);
-        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+        const Two d = add2(t, Two{-f.x, -f.y});
+        const __half2 r = __floats2half2_rn(d.x, d.y);
         h[i] = *reinterpret_cast<const unsigned*>(&p), l[i] = *reinterpret_cast<const unsigned*>(&r);
     }
     hi = make_uint4(h[0], h[1], h[2], h[3]), lo = make_uint4(l[0], l[1], l[2], l[3]);
@@ -182,12 +181,10 @@ __device__ __forceinline__ void block_colsum(const Eight (&x)[2], float (&buf)[8
     }
 }
 
-// Eight columns of `row` of a job's operand, in fp32 or from its checkpoint.
-__device__ __forceinline__ Eight load8_held(const PackJob& j, const float* p, const void* ck, int64_t row, int64_t col, int have) {
+// Eight columns from element `off`, group `group` on, of a job's operand in fp32 or (ck not null) of its checkpoint.
+__device__ __forceinline__ Eight load8_held(const float* p, const void* ck, const unsigned char* exp, int wide, int64_t off, int64_t group, int have) {
     if (have == 0) return load8(nullptr, 0, false);
-    const bool whole = (j.cols & 7) == 0;
-    return ck ? load8_ck(ck, j.rows, j.cols, row, col, have, whole && (reinterpret_cast<uintptr_t>(ck) & 7) == 0)
-              : load8(p + row * j.cols + col, have, whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0);
+    return ck ? load8_ck(static_cast<const signed char*>(ck) + off, exp + group, have, wide) : load8(p + off, have, wide);
 }
 
 // One block of 64 x 64: a thread takes eight columns of two rows, all of whose loads are issued before the first is used.
@@ -203,22 +200,30 @@ __device__ __forceinline__ void pack_unit(const PackJob& j, int unit, float scal
     unsigned most = 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int64_t row = (int64_t)rb * kBlock + row_in + 32 * h;
+        const int64_t row = (int64_t)rb * kBlock + row_in + 32 * h, off = row * j.cols + col;
+        const int64_t group = KIND == PACK_FP32 ? 0 : row * j.groups + col / kGroup;
         const int got = row < j.rows ? have : 0;
-        x[h] = load8_held(j, j.a, KIND == PACK_CK8 ? j.b8 : nullptr, row, col, got);
-        if (KIND == PACK_ACT || KIND == PACK_GATED) y[h] = load8_held(j, j.b, j.b8, row, col, got);
-        if (KIND == PACK_GATED) z[h] = load8_held(j, j.c, j.c8, row, col, got);
+        if (KIND == PACK_CK8) x[h] = load8_held(nullptr, j.b8, j.b_exp, j.b_wide, off, group, got);
+        else x[h] = load8_held(j.a, nullptr, nullptr, j.a_wide, off, 0, got);
+        if (KIND == PACK_ACT || KIND == PACK_GATED) y[h] = load8_held(j.b, j.b8, j.b_exp, j.b_wide, off, group, got);
+        if (KIND == PACK_GATED) z[h] = load8_held(j.c, j.c8, j.c_exp, j.c_wide, off, group, got);
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int r = row_in + 32 * h;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (KIND == PACK_ACT) x[h].v[i] *= act_grad(j.act, y[h].v[i]);
+        for (int i = 0; i < 8; i += 2) {
+            const Two d = Two{x[h].v[i], x[h].v[i + 1]}, pre = Two{y[h].v[i], y[h].v[i + 1]};
+            if (KIND == PACK_ACT) {
+                const Two r = mul2(d, act_grad2(j.act, pre));
+                x[h].v[i] = r.x, x[h].v[i + 1] = r.y;
+            }
             if (KIND == PACK_GATED) {
-                const float d = x[h].v[i], gate = y[h].v[i];
-                x[h].v[i] = d * z[h].v[i] * act_grad(j.act, gate);
-                y[h].v[i] = d * act_of(j.act, gate);
+                Two value, grad;
+                act_and_grad2(j.act, pre, value, grad);
+                const Two r = mul2(mul2(d, Two{z[h].v[i], z[h].v[i + 1]}), grad), up = mul2(d, value);
+                x[h].v[i] = r.x, x[h].v[i + 1] = r.y;
+                y[h].v[i] = up.x, y[h].v[i + 1] = up.y;
             }
         }
         if (TOP && KIND != PACK_CK8) {
@@ -409,7 +414,21 @@ static dim3 pack_grid(const PackArgs& a, int sm_count) {
     const int most = sm_count * (gated(a) ? kPackPerSM<true> : kPackPerSM<false>);  // as many as run at once: each starts with the maxima
     return dim3((unsigned)(a.units < most ? a.units : most));
 }
-cudaError_t launch_pack(const PackArgs& a, int sm_count, cudaStream_t st) {
+static void set_access(PackArgs& a) {
+    const auto aligned = [](const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+    for (int i = 0; i < a.jobs; i++) {
+        PackJob& j = a.job[i];
+        const bool whole = (j.cols & 7) == 0;
+        j.groups = ck8_groups(j.cols);
+        j.a_wide = whole && aligned(j.a, 16);
+        j.b_wide = whole && (j.b8 ? aligned(j.b8, 8) : aligned(j.b, 16));
+        j.c_wide = whole && (j.c8 ? aligned(j.c8, 8) : aligned(j.c, 16));
+        j.b_exp = j.b8 ? static_cast<const unsigned char*>(j.b8) + ck8_exp_offset(j.rows, j.cols) : nullptr;
+        j.c_exp = j.c8 ? static_cast<const unsigned char*>(j.c8) + ck8_exp_offset(j.rows, j.cols) : nullptr;
+    }
+}
+cudaError_t launch_pack(PackArgs& a, int sm_count, cudaStream_t st) {
+    set_access(a);
     const auto kernel = gated(a) ? (a.sampled ? k_pack<true, true> : k_pack<false, true>) : (a.sampled ? k_pack<true, false> : k_pack<false, false>);
     return launch_early(kernel, pack_grid(a, sm_count), kThreads, 0, st, 1, a);
 }
