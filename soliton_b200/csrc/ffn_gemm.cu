@@ -148,7 +148,10 @@ __device__ __forceinline__ void tmem_add16(unsigned addr, float gain, float* sum
                  : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; i++) sum[i] = fmaf(__uint_as_float(r[i]), gain, sum[i]);
+    for (int i = 0; i < 16; i += 2) {
+        const Two t = fma2(Two{__uint_as_float(r[i]), __uint_as_float(r[i + 1])}, both(gain), Two{sum[i], sum[i + 1]});
+        sum[i] = t.x, sum[i + 1] = t.y;
+    }
 }
 
 // Shared-memory descriptors of blocks (128-byte swizzle; groups of eight 128-byte rows lie 1 KiB apart for each piece).
@@ -257,8 +260,9 @@ __device__ __forceinline__ void scale_row(float (&v)[32], float row, const float
     for (int i = 0; i < 32; i += 4) {
         const float4 c = *reinterpret_cast<const float4*>(col + i);
         const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        v[i] = fmaf(v[i] * row, c.x, b.x), v[i + 1] = fmaf(v[i + 1] * row, c.y, b.y);
-        v[i + 2] = fmaf(v[i + 2] * row, c.z, b.z), v[i + 3] = fmaf(v[i + 3] * row, c.w, b.w);
+        const Two x = fma2(mul2(Two{v[i], v[i + 1]}, both(row)), Two{c.x, c.y}, Two{b.x, b.y});
+        const Two y = fma2(mul2(Two{v[i + 2], v[i + 3]}, both(row)), Two{c.z, c.w}, Two{b.z, b.w});
+        v[i] = x.x, v[i + 1] = x.y, v[i + 2] = y.x, v[i + 3] = y.y;
     }
 }
 template <int ACT>
