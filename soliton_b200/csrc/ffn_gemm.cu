@@ -1,15 +1,15 @@
 // fp32-class matrix products over operand planes (ffn.hpp) on the fifth-generation tensor cores.
 //
 // D = A * B^T over blocks of 64 along K. Per k-block a stage of shared memory receives the blocks of both operands by
-// bulk copies (each block is the 8 KiB image the tensor cores read, so a stage is a handful of contiguous copies and no
-// tensor map is needed, whatever the matrix's sizes), and one thread issues the products hi*hi, hi*lo, lo*hi of 128 x BN
-// x 16 each into an accumulator in tensor memory. K-major and MN-major operands read the same image through different
-// descriptors.
+// bulk copies (each block is the image the tensor cores read, so a stage is a handful of contiguous copies and no tensor map
+// is needed, whatever the matrix's sizes), and one thread issues the products lo*hi, hi*hi, hi*lo, 16 terms each, into an
+// accumulator in tensor memory. K-major and MN-major operands read the same image through different descriptors.
 //
 // The tensor cores round every accumulation towards zero, so a long sum drifts, by 0.14 ulps a step on the average. That
-// much is given back (segment_gain), and sums are cut into segments of 256 to 384 along K: the accumulator has two buffers, the warps of the epilogue add a finished
-// segment to fp32 registers (to nearest) while the next one runs in the other buffer. The same double buffer lets a
-// tile's epilogue run under the next tile's products: blocks are persistent, one per SM.
+// much is given back (segment_gain), and sums are cut into segments of 256 to 384 terms: the accumulator has two buffers, the
+// warps of the epilogue add a finished segment to fp32 registers (to nearest) while the next one runs in the other
+// buffer. The same double buffer lets a tile's epilogue run under the next tile's products: blocks are persistent, one per
+// SM. At 4096 x 4096 x 4096 a tile takes 106 to 120 k cycles, its products alone 98 k.
 //
 // The epilogue works on the accumulator's own arrangement, a row per lane and 32 columns at a time (one group of a
 // checkpoint), and turns pieces of 32 x 32 through shared memory to store them in whole lines.
