@@ -468,36 +468,41 @@ __device__ __forceinline__ Piece rows_of(const GemmArgs& g, int m, int rank, int
     return p;
 }
 
-// The slices' sums, a warp per 32 x 32 results: grid over tiles, then parts of a tile, then chunks.
-constexpr int kSliceWarps = 4;
+// The slices' sums, a warp per 32 rows of eight results, a row per lane: grid over tiles, then parts of a tile, then eights.
+// (A warp per 32 x 32 left most SMs without work: 14 us for sixteen slices of 32 tiles.)
+constexpr int kSliceThreads = 128;
 template <int CTAS>
-__global__ void __launch_bounds__(32 * kSliceWarps) k_slices(const __grid_constant__ GemmArgs g) {
-    constexpr int kChunks = 2 * CTAS, kWarps = CTAS * kEpiWarps;
-    __shared__ alignas(16) float turn_buf[kSliceWarps][kTurnFloats];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(kSliceThreads) k_slices(const __grid_constant__ GemmArgs g) {
+    constexpr int kEights = 8 * CTAS, kWarps = CTAS * kEpiWarps;
+    const int lane = threadIdx.x & 31;
     stream_next();
     stream_wait();
-    const int unit = (int)blockIdx.x * kSliceWarps + warp, c = unit % kChunks, who = unit / kChunks % kWarps, tile = unit / (kChunks * kWarps);
+    const int unit = (int)blockIdx.x * (kSliceThreads / 32) + (threadIdx.x >> 5), e = unit % kEights, who = unit / kEights % kWarps, tile = unit / (kEights * kWarps);
     const Unit at = unit_at(tile * g.slices, g);
-    const int rank = who / kEpiWarps, q = who & 3, half = who / 4 % 2;
-    Piece p = rows_of<CTAS, EPI_STORE>(g, at.m, rank, q);
-    p.col0 = (int64_t)at.n * 128 * CTAS + (half * kChunks + c) * 32;
-    if (p.rows == 0 || p.col0 >= g.cols) return;
-    float v[32], s1, s2;
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < g.slices; s++) {
-        const float4* from = slice_place<kChunks>(g.partial, tile * g.slices + s, kWarps, who, lane) + c * 256;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float4 x = __ldcg(from + i * 32);
-            v[4 * i] += x.x, v[4 * i + 1] += x.y, v[4 * i + 2] += x.z, v[4 * i + 3] += x.w;
-        }
+    const Piece p = rows_of<CTAS, EPI_STORE>(g, at.m, who / kEpiWarps, who & 3);
+    const int64_t col = (int64_t)at.n * 128 * CTAS + (who / 4 % 2) * 64 * CTAS + e * 8;
+    if (lane >= p.rows || col >= g.cols) return;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    const float4* from = slice_place<2 * CTAS>(g.partial, tile * g.slices, kWarps, who, lane) + e * 64;
+#pragma unroll 8
+    for (int s = 0; s < g.slices; s++, from += kWarps * (2 * CTAS * 256)) {
+        const float4 x = __ldcg(from), y = __ldcg(from + 32);
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
     }
+    float s1, s2;
     plane_scales(g, s1, s2);
-    if (g.wide && p.col0 + 32 <= g.cols) finish_wide<EPI_STORE>(g, v, v, p, s1, s2, turn_buf[warp], lane);
-    else finish_any<EPI_STORE>(g, v, v, p, s1, s2, turn_buf[warp], lane);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = v[i] * s1 * s2;
+    const bool second = p.row0 >= g.split;
+    float* out = (second ? g.out2 : g.out) + (p.row0 + lane - (second ? g.split : 0)) * g.cols + col;
+    if (g.wide && col + 8 <= g.cols) {
+        *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(out + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (col + i < g.cols) out[i] = v[i];
+    }
 }
 
 // CTAS = 1: a block per tile of 128 x 128. CTAS = 2: a pair of blocks (a cluster) per tile of 256 x 256: each holds 128 rows of A
@@ -767,8 +772,8 @@ static cudaError_t launch_one(const GemmArgs& g, int sm_count, cudaStream_t st) 
     const int units = g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices, teams = sm_count / CTAS;
     const cudaError_t rc = launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
     if (rc != cudaSuccess || !later(EPI, g.slices)) return rc;
-    const int cut = g.m_tiles * g.n_tiles - g.whole;  // of CTAS x kEpiWarps parts of 2 CTAS chunks each
-    return launch_early(k_slices<CTAS>, dim3((unsigned)(cut * CTAS * kEpiWarps * 2 * CTAS / kSliceWarps)), 32 * kSliceWarps, 0, st, 1, g);
+    const int cut = g.m_tiles * g.n_tiles - g.whole;  // of CTAS x kEpiWarps parts of 8 CTAS eights each
+    return launch_early(k_slices<CTAS>, dim3((unsigned)(cut * CTAS * kEpiWarps * 8 * CTAS / (kSliceThreads / 32))), kSliceThreads, 0, st, 1, g);
 }
 template <int PB, bool AMN, bool BMN, int EPI>
 static cudaError_t launch_sized(GemmArgs& g, int sm_count, cudaStream_t st) {

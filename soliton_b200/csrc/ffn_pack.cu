@@ -316,12 +316,13 @@ __global__ void __launch_bounds__(kThreads, kPackPerSM<GATED>) k_repack(const __
 }
 static_assert(kMaxPlanes == 3, "three planes by name above");
 
-// Planes with a scale for each row: a warp takes a row, holds it in registers between its maximum and its pieces (CHUNKS
-// times 256 values; a longer row is read again, from L2), and a block the eight rows of a group.
-template <int CHUNKS>
-__device__ __forceinline__ void pack_row(const RowJob& j, int64_t row, int lane) {
+// Planes with a scale for each row: WARPS warps take a row and hold it in registers between its maximum and its pieces
+// (CHUNKS times 256 values each; with 0, for rows that would not fit, it is read again, from L2). A block takes 8 / WARPS rows.
+template <int CHUNKS, int WARPS>
+__device__ __forceinline__ void pack_row(const RowJob& j, int64_t row, int part, unsigned* tops) {
+    const int lane = threadIdx.x & 31;
     const bool wide = (j.cols & 7) == 0 && (reinterpret_cast<uintptr_t>(j.a) & 15) == 0;
-    const int chunks = j.col_blocks * 8;
+    const int chunks = j.col_blocks * 8, first = part * 32 + lane;
     const float* src = j.a + row * j.cols;
     const bool there = row < j.rows;
     const auto fetch = [&](int c) {
@@ -332,44 +333,68 @@ __device__ __forceinline__ void pack_row(const RowJob& j, int64_t row, int lane)
     unsigned top = 0;
     if (CHUNKS > 0) {
 #pragma unroll
-        for (int i = 0; i < CHUNKS; i++) x[i] = fetch(lane + 32 * i);
+        for (int i = 0; i < CHUNKS; i++) x[i] = fetch(first + 32 * WARPS * i);
 #pragma unroll
         for (int i = 0; i < CHUNKS; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) top = max(top, finite_bits(x[i].v[e]));
     } else {
 #pragma unroll 4
-        for (int c = lane; c < chunks; c += 32) {
+        for (int c = first; c < chunks; c += 32 * WARPS) {
             const Eight y = fetch(c);
 #pragma unroll
             for (int e = 0; e < 8; e++) top = max(top, finite_bits(y.v[e]));
         }
     }
     top = __reduce_max_sync(0xffffffffu, top);
+    if (WARPS > 1) {
+        const int warp = threadIdx.x >> 5;
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) top = max(top, tops[warp / WARPS * WARPS + w]);
+    }
     const int e = min(max(exponent_of(top, 0), kLeastExp), kMostExp);
     const float scale = exp2f((float)(15 - e));
-    if (lane == 0) j.factor[row] = exp2f((float)(j.is_a ? e - 30 : e));
+    if (first == 0) j.factor[row] = exp2f((float)(j.is_a ? e - 30 : e));
     char* base = j.plane + (row >> 6) * j.col_blocks * (int64_t)(2 * kImageBytes);
     const auto put = [&](int c, const Eight& y) { store_pieces(base + (int64_t)(c >> 3) * (int64_t)(2 * kImageBytes), 2, (int)(row & 63), c & 7, y, scale); };
     if (CHUNKS > 0) {
 #pragma unroll
         for (int i = 0; i < CHUNKS; i++)
-            if (lane + 32 * i < chunks) put(lane + 32 * i, x[i]);
+            if (first + 32 * WARPS * i < chunks) put(first + 32 * WARPS * i, x[i]);
     } else {
 #pragma unroll 4
-        for (int c = lane; c < chunks; c += 32) put(c, fetch(c));
+        for (int c = first; c < chunks; c += 32 * WARPS) put(c, fetch(c));
     }
 }
-template <int CHUNKS>
+template <int CHUNKS, int WARPS>
 __global__ void __launch_bounds__(kThreads) k_rows(const __grid_constant__ RowArgs a) {
+    __shared__ unsigned tops[kThreads / 32];
     stream_next();
     stream_wait();
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < a.n_counters; i += kThreads) a.counters[i] = 0;
+    const int group = (int)blockIdx.x / WARPS, warp = threadIdx.x >> 5;
     int ji = a.jobs - 1;
-    while ((int)blockIdx.x < a.job[ji].first_group) ji--;
+    while (group < a.job[ji].first_group) ji--;
     const RowJob& j = a.job[ji];
-    pack_row<CHUNKS>(j, (int64_t)((int)blockIdx.x - j.first_group) * 8 + (threadIdx.x >> 5), threadIdx.x & 31);
+    pack_row<CHUNKS, WARPS>(j, (int64_t)(group - j.first_group) * 8 + (int)blockIdx.x % WARPS * (8 / WARPS) + warp / WARPS, warp % WARPS, tops);
+}
+struct RowKernel {
+    void (*kernel)(RowArgs);
+    int warps;
+};
+// By the row's blocks of 64 columns, four to a chunk of 256 (8192 x 4096: 64 us read twice by a warp, 38 once by four).
+static RowKernel row_kernel(int blocks) {
+    if (blocks <= 4) return {k_rows<1, 1>, 1};
+    if (blocks <= 8) return {k_rows<2, 1>, 1};
+    if (blocks <= 12) return {k_rows<3, 1>, 1};
+    if (blocks <= 16) return {k_rows<4, 1>, 1};
+    if (blocks <= 32) return {k_rows<4, 2>, 2};
+    if (blocks <= 64) return {k_rows<4, 4>, 4};
+    if (blocks <= 128) return {k_rows<4, 8>, 8};
+    return {k_rows<0, 8>, 8};
 }
 
 // A block takes 32 columns, each of its warps every eighth block row; the eight sums meet in order.
@@ -396,9 +421,8 @@ __global__ void __launch_bounds__(kThreads) k_colsum(const float* parts, float* 
 }
 
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t st) {
-    const int blocks = a.job[0].col_blocks;  // of 64 columns: four to a chunk of 256; all jobs have the same
-    const auto kernel = blocks <= 4 ? k_rows<1> : blocks <= 8 ? k_rows<2> : blocks <= 12 ? k_rows<3> : blocks <= 16 ? k_rows<4> : blocks <= 32 ? k_rows<8> : k_rows<0>;
-    return launch_early(kernel, dim3((unsigned)a.groups), kThreads, 0, st, 1, a);
+    const RowKernel k = row_kernel(a.job[0].col_blocks);  // all jobs have the same
+    return launch_early(k.kernel, dim3((unsigned)(a.groups * k.warps)), kThreads, 0, st, 1, a);
 }
 
 cudaError_t launch_amax(const AmaxArgs& a, int, cudaStream_t st) {

@@ -10,8 +10,8 @@ from tests.gpu_util import CUDA, DevBuf, check_ok
 
 pytestmark = [pytest.mark.gpu, pytest.mark.usefixtures("cuda")]
 
-# (m, n, k); three run their forward product, input gradient and weight gradient in pairs of blocks; the last has rows that do not fit registers
-SIZES = [(1, 1, 1), (2, 3, 5), (1, 300, 40), (64, 128, 32), (65, 63, 64), (128, 256, 64), (129, 257, 65), (333, 515, 257), (70, 130, 1100), (260, 190, 515), (1700, 1300, 200), (1700, 40, 1300), (40, 1700, 1300), (70, 90, 2500)]
+# (m, n, k); three run their forward product, input gradient and weight gradient in pairs of blocks; then rows that several warps hold, and that do not fit registers
+SIZES = [(1, 1, 1), (2, 3, 5), (1, 300, 40), (64, 128, 32), (65, 63, 64), (128, 256, 64), (129, 257, 65), (333, 515, 257), (70, 130, 1100), (260, 190, 515), (1700, 1300, 200), (1700, 40, 1300), (40, 1700, 1300), (70, 90, 2500), (20, 30, 6000), (9, 20, 9000)]
 
 
 def normal(rng, *shape, std=1.0):
