@@ -138,6 +138,8 @@ struct GemmPlan {
 };
 // store: a plain product (EPI_STORE)
 GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks, bool store);
+// Whether two plain products are small enough to run in one launch, on SMs of their own.
+bool side_by_side(const GemmPlan& dx, const GemmPlan& dw);
 
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t st);
 cudaError_t launch_amax(const AmaxArgs& a, int sm_count, cudaStream_t st);
@@ -146,6 +148,9 @@ cudaError_t launch_pack(PackArgs& a, int sm_count, cudaStream_t st);
 cudaError_t launch_repack(const PackArgs& a, int sm_count, cudaStream_t st);
 // out[j] = the sum over `parts` of the block rows' column sums, in order; the same for a second matrix where given
 cudaError_t launch_colsum(const float* parts, float* out, const float* parts2, float* out2, int count, int64_t cols, cudaStream_t st);
+// dx (A K-major, B MN-major) and dw (both MN-major) in one launch, where side_by_side() says so; they need partial sums and
+// counters of their own.
+cudaError_t launch_gemm_pair(const GemmArgs& dx, const GemmArgs& dw, int pieces_b, cudaStream_t st, int& launches);
 // a_mn, b_mn: the operand's blocks hold K along their rows. pieces_b: 1 when B is a checkpoint's plane.
 cudaError_t launch_gemm(const GemmArgs& g, bool a_mn, bool b_mn, int pieces_b, Epilogue epi, int sm_count, cudaStream_t st);
 

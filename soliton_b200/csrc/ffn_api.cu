@@ -69,7 +69,7 @@ size_t carve(Scratch& s, void* base, int64_t m, int64_t n, int64_t k, int weight
         s.colsum = reinterpret_cast<float*>(c.take((size_t)(mb * n) * sizeof(float)));
         s.colsum2 = weights == 2 ? reinterpret_cast<float*>(c.take((size_t)(mb * n) * sizeof(float))) : nullptr;
         s.n_counters = dx.counters + dw_counters;
-        partial = dx.partial_bytes > dw.partial_bytes ? dx.partial_bytes : dw.partial_bytes;
+        partial = side_by_side(dx, dw) ? dx.partial_bytes + dw.partial_bytes : dx.partial_bytes > dw.partial_bytes ? dx.partial_bytes : dw.partial_bytes;
         if (half.partial_bytes > partial) partial = half.partial_bytes;  // one of the gated pair's weights alone
     } else {
         const GemmPlan p = gemm_plan(mb, weights * nb, kb, false);
@@ -108,9 +108,9 @@ public:
     void writes(void* p, int64_t bytes) {
         if (p && bytes > 0) e_.legacy_touches(p, (size_t)bytes, true);
     }
-    void launched(cudaError_t rc) {
+    void launched(cudaError_t rc, int count = 1) {
         if (rc != cudaSuccess) failed_ = true;
-        count_++;
+        count_ += count;
     }
     int done() {
         e_.legacy_launches(count_);
@@ -255,23 +255,25 @@ int run_gated(const float* x, const float* wg, const float* wu, const float* bg,
 // by side (`width` blocks in all).
 void gradients(Op& op, const Scratch& s, bool x_ck8, float* dx, float* dw, float* dw2, int64_t m, int64_t n, int64_t k, int halves) {
     const int64_t mb = blocks_of(m), nb = blocks_of(n), kb = blocks_of(k), width = halves * nb;
-    if (dx) {
-        GemmArgs g = product(op, s);
-        g.a = k_major(s.y, mb, width, PLANE_Y), g.b = mn_major(s.w, kb, kb, PLANE_W);
-        g.k_blocks = (int)width, g.k_len = halves == 2 ? width * kBlock : n, g.rows = m, g.cols = k, g.out = dx;
-        op.launched(launch_gemm(g, false, true, 2, EPI_STORE, op.sms(), 0));
+    const GemmPlan dx_plan = gemm_plan(mb, kb, width, true);
+    const bool both = dw && dw2, whole = halves == 1 || both;  // or one of the gated pair alone: its half of the plane
+    GemmArgs x = product(op, s), w = product(op, s);
+    x.a = k_major(s.y, mb, width, PLANE_Y), x.b = mn_major(s.w, kb, kb, PLANE_W);
+    x.k_blocks = (int)width, x.k_len = halves == 2 ? width * kBlock : n, x.rows = m, x.cols = k, x.out = dx;
+    w.counters += dx_plan.counters;
+    w.a = mn_major(s.y + (whole || dw ? 0 : nb * (int64_t)(2 * kImageBytes)), whole ? width : nb, width, PLANE_Y), w.b = mn_major(s.x, kb, kb, PLANE_X);
+    w.k_blocks = (int)mb, w.k_len = m, w.rows = n, w.cols = k, w.out = dw ? dw : dw2;
+    if (both) w.split = nb * kBlock, w.out2 = dw2;
+    const int pieces = x_ck8 ? 1 : 2;
+    if (dx && (dw || dw2) && whole && side_by_side(dx_plan, gemm_plan(width, kb, mb, true))) {
+        w.partial += dx_plan.partial_bytes / sizeof(float);
+        int launches = 0;
+        const cudaError_t rc = launch_gemm_pair(x, w, pieces, 0, launches);
+        op.launched(rc, launches);
+        return;
     }
-    if (dw || dw2) {
-        // one of the gated pair alone: its half of the plane
-        const bool both = dw && dw2;
-        const char* y = s.y + (halves == 2 && !dw ? nb * (int64_t)(2 * kImageBytes) : 0);
-        GemmArgs g = product(op, s);
-        g.counters += gemm_plan(mb, kb, width, true).counters;  // behind dx's
-        g.a = mn_major(y, both ? width : nb, width, PLANE_Y), g.b = mn_major(s.x, kb, kb, PLANE_X);
-        g.k_blocks = (int)mb, g.k_len = m, g.rows = n, g.cols = k, g.out = dw ? dw : dw2;
-        if (both) g.split = nb * kBlock, g.out2 = dw2;
-        op.launched(launch_gemm(g, true, true, x_ck8 ? 1 : 2, EPI_STORE, op.sms(), 0));
-    }
+    if (dx) op.launched(launch_gemm(x, false, true, 2, EPI_STORE, op.sms(), 0));
+    if (dw || dw2) op.launched(launch_gemm(w, true, true, pieces, EPI_STORE, op.sms(), 0));
 }
 void no_rows(Op& op, float* p, int64_t count) {  // a sum over no rows
     if (p) op.launched(cudaMemsetAsync(p, 0, (size_t)count * 4, 0));

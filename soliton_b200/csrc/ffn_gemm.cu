@@ -510,8 +510,9 @@ __global__ void __launch_bounds__(kSliceThreads) k_slices(const __grid_constant_
 // read both. Per value fetched a pair computes twice as much, which is what bounds large products: fetching from L2.
 // Warp 0 copies, warp 1 issues the products (in a pair's second block: reports arrived stages to the first), warps 4 to
 // 11 read the accumulators: two per 32 rows, half the columns each.
+// `block` of `blocks`: of those that work on this product.
 template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
-__global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs g) {
+__device__ __forceinline__ void multiply(const GemmArgs& g, int block, int blocks) {
     constexpr int BN = 128 * CTAS, kBlocksN = BN / kBlock, kChunks = BN / 64;  // chunks of 32 columns a warp
     constexpr unsigned kABlock = 2 * (unsigned)kImageBytes, kBBlock = PB * (unsigned)kImageBytes;
     constexpr int kStageBytes = 2 * (kABlock + kBBlock);  // this block's 128 rows of A and its share of B
@@ -526,8 +527,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     const unsigned full = bar_at, empty = full + 8 * kMaxStages, peer_full = empty + 8 * kMaxStages, tfull = peer_full + 8 * kMaxStages, tempty = tfull + 16,
                    drained = tempty + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;
-    const int team = (int)blockIdx.x / CTAS, teams = (int)gridDim.x / CTAS;
+    const int rank = CTAS == 2 ? block & 1 : 0;
+    const int team = block / CTAS, teams = blocks / CTAS;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; s++) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 1), mbar_init(peer_full + 8 * s, 1);
@@ -729,6 +730,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant_
     }
 }
 
+template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
+__global__ void __launch_bounds__(kGemmThreads, 1) k_gemm(const __grid_constant__ GemmArgs g) {
+    multiply<CTAS, PB, AMN, BMN, EPI>(g, (int)blockIdx.x, (int)gridDim.x);
+}
+// dx and dw of a small layer side by side: `first` blocks for dx, the others for dw.
+template <int PB>
+__global__ void __launch_bounds__(kGemmThreads, 1) k_both(const __grid_constant__ GemmArgs dx, const __grid_constant__ GemmArgs dw, int first) {
+    if ((int)blockIdx.x < first) multiply<1, 2, false, true, EPI_STORE>(dx, (int)blockIdx.x, first);
+    else multiply<1, PB, true, true, EPI_STORE>(dw, (int)blockIdx.x - first, (int)gridDim.x - first);
+}
+
 // ---------------------------------------------------------------- how a product is cut
 
 // Estimated cycles of a way of cutting: rounds of whole tiles, then rounds of slices. A k-block takes a pair 1,750 cycles,
@@ -765,37 +777,70 @@ GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks, bool st
     return best;
 }
 
-template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
-static cudaError_t launch_one(const GemmArgs& g, int sm_count, cudaStream_t st) {
-    static const cudaError_t ready = cudaFuncSetAttribute(k_gemm<CTAS, PB, AMN, BMN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-    if (ready != cudaSuccess) return ready;
-    const int units = g.whole + (g.m_tiles * g.n_tiles - g.whole) * g.slices, teams = sm_count / CTAS;
-    const cudaError_t rc = launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
-    if (rc != cudaSuccess || !later(EPI, g.slices)) return rc;
+static int unit_count(const GemmPlan& p) { return p.whole + (p.m_tiles * p.n_tiles - p.whole) * p.slices; }
+bool side_by_side(const GemmPlan& dx, const GemmPlan& dw) { return dx.ctas == 1 && dw.ctas == 1 && unit_count(dx) + unit_count(dw) <= kPlanSMs; }
+
+static GemmPlan set_plan(GemmArgs& g, bool gated, bool store) {
+    const GemmPlan p = gemm_plan(g.a.mn_blocks, gated ? 2 * (int64_t)g.gate_blocks : g.b.mn_blocks, g.k_blocks, store);
+    g.m_tiles = p.m_tiles, g.n_tiles = p.n_tiles, g.whole = p.whole, g.slices = p.slices;
+    return p;
+}
+template <class Kernel>
+static cudaError_t allow_shared(Kernel kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes); }
+template <int CTAS>
+static cudaError_t launch_slices(const GemmArgs& g, cudaStream_t st) {
     const int cut = g.m_tiles * g.n_tiles - g.whole;  // of CTAS x kEpiWarps parts of 8 CTAS eights each
     return launch_early(k_slices<CTAS>, dim3((unsigned)(cut * CTAS * kEpiWarps * 8 * CTAS / (kSliceThreads / 32))), kSliceThreads, 0, st, 1, g);
 }
+template <int CTAS, int PB, bool AMN, bool BMN, int EPI>
+static cudaError_t launch_one(const GemmArgs& g, int units, int sm_count, cudaStream_t st) {
+    static const cudaError_t ready = allow_shared(k_gemm<CTAS, PB, AMN, BMN, EPI>);
+    if (ready != cudaSuccess) return ready;
+    const int teams = sm_count / CTAS;
+    const cudaError_t rc = launch_early(k_gemm<CTAS, PB, AMN, BMN, EPI>, dim3((unsigned)(CTAS * (units < teams ? units : teams))), kGemmThreads, kSmemBytes, st, CTAS, g);
+    return rc != cudaSuccess || !later(EPI, g.slices) ? rc : launch_slices<CTAS>(g, st);
+}
 template <int PB, bool AMN, bool BMN, int EPI>
 static cudaError_t launch_sized(GemmArgs& g, int sm_count, cudaStream_t st) {
-    const GemmPlan p = gemm_plan(g.a.mn_blocks, EPI == EPI_GATED ? 2 * (int64_t)g.gate_blocks : g.b.mn_blocks, g.k_blocks, EPI == EPI_STORE);
-    g.m_tiles = p.m_tiles, g.n_tiles = p.n_tiles, g.whole = p.whole, g.slices = p.slices;
-    return p.ctas == 1 ? launch_one<1, PB, AMN, BMN, EPI>(g, sm_count, st) : launch_one<2, PB, AMN, BMN, EPI>(g, sm_count, st);
+    const GemmPlan p = set_plan(g, EPI == EPI_GATED, EPI == EPI_STORE);
+    return p.ctas == 1 ? launch_one<1, PB, AMN, BMN, EPI>(g, unit_count(p), sm_count, st) : launch_one<2, PB, AMN, BMN, EPI>(g, unit_count(p), sm_count, st);
+}
+template <int PB>
+static cudaError_t launch_pair(const GemmArgs& dx, int dx_units, const GemmArgs& dw, int dw_units, cudaStream_t st) {
+    static const cudaError_t ready = allow_shared(k_both<PB>);
+    if (ready != cudaSuccess) return ready;
+    return launch_early(k_both<PB>, dim3((unsigned)(dx_units + dw_units)), kGemmThreads, kSmemBytes, st, 1, dx, dw, dx_units);
 }
 
 static bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-cudaError_t launch_gemm(const GemmArgs& args, bool a_mn, bool b_mn, int pieces_b, Epilogue epi, int sm_count, cudaStream_t st) {
-    GemmArgs g = args;
+static void set_access(GemmArgs& g) {
     const bool ck = g.save8 || g.save8_2;
     g.wide = g.cols % (ck ? 8 : 4) == 0 && aligned(g.out, 16) && aligned(g.out2, 16) && aligned(g.bias, 16) && aligned(g.bias2, 16) &&
              aligned(g.residual, 16) && aligned(g.save, 16) && aligned(g.save2, 16) && aligned(g.save8, 8) && aligned(g.save8_2, 8);
     g.groups = ck8_groups(g.cols), g.exp_offset = ck8_exp_offset(g.rows, g.cols);
+}
+
+cudaError_t launch_gemm(const GemmArgs& args, bool a_mn, bool b_mn, int pieces_b, Epilogue epi, int sm_count, cudaStream_t st) {
+    GemmArgs g = args;
+    set_access(g);
     if (epi == EPI_LINEAR) return launch_sized<2, false, false, EPI_LINEAR>(g, sm_count, st);
     if (epi == EPI_GATED) return launch_sized<2, false, false, EPI_GATED>(g, sm_count, st);
     if (!a_mn && b_mn) return launch_sized<2, false, true, EPI_STORE>(g, sm_count, st);
     if (a_mn && b_mn && pieces_b == 2) return launch_sized<2, true, true, EPI_STORE>(g, sm_count, st);
     if (a_mn && b_mn && pieces_b == 1) return launch_sized<1, true, true, EPI_STORE>(g, sm_count, st);
     return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_gemm_pair(const GemmArgs& dx_args, const GemmArgs& dw_args, int pieces_b, cudaStream_t st, int& launches) {
+    GemmArgs dx = dx_args, dw = dw_args;
+    set_access(dx), set_access(dw);
+    const GemmPlan px = set_plan(dx, false, true), pw = set_plan(dw, false, true);
+    launches = 1;
+    cudaError_t rc = pieces_b == 1 ? launch_pair<1>(dx, unit_count(px), dw, unit_count(pw), st) : launch_pair<2>(dx, unit_count(px), dw, unit_count(pw), st);
+    if (rc == cudaSuccess && later(EPI_STORE, dx.slices)) rc = launch_slices<1>(dx, st), launches++;
+    if (rc == cudaSuccess && later(EPI_STORE, dw.slices)) rc = launch_slices<1>(dw, st), launches++;
+    return rc;
 }
 
 }  // namespace slb_ffn
