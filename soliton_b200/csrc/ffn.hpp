@@ -138,7 +138,7 @@ struct GemmPlan {
 };
 // store: a plain product (EPI_STORE)
 GemmPlan gemm_plan(int64_t m_blocks, int64_t n_blocks, int64_t k_blocks, bool store);
-// Whether two plain products are small enough to run in one launch, on SMs of their own.
+// Whether two plain products are small enough to run in one launch: blocks of one tile or slice each, two an SM at the most.
 bool side_by_side(const GemmPlan& dx, const GemmPlan& dw);
 
 cudaError_t launch_rows(const RowArgs& a, cudaStream_t st);
